@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define BSMM_ABI_VERSION 2
+#define BSMM_ABI_VERSION 3
 
 /* status codes */
 #define BSMM_OK 0
@@ -292,6 +292,68 @@ int bsmm_move_blocks(int32_t* blocks, const int32_t* slots, const int32_t* cells
 int bsmm_sddmm_static(const void* a, const void* b, int64_t rows, int64_t cols, int64_t tokens, float* sparse_c,
                       const int32_t* blocks, int64_t nnz, const int32_t* csr_idx, const void* plan,
                       float* block_sumsq, uint32_t flags, bsmm_stream_t stream);
+
+/*
+ * Operators around a block-sparse projection.  No counterpart in the reference.
+ *
+ * The gated feed-forward block, h = act(g) * u with g = x Wg^T + bg and u = x Wu^T + bu.  Wg and Wu [hidden, k] are ONE
+ * block-sparse matrix of 2 * hidden rows whose block-rows alternate: block-row 2j is Wg's block-row j, 2j + 1 is Wu's.
+ * Its products (bsmm_dsd, bsmm_sddmm) then work on pre-activations `pre` [m, 2 * hidden] whose columns alternate the same
+ * way: 32 columns of g, 32 of u, and so on.  hidden is a multiple of 32; m is free (0 is a no-op).
+ *   bsmm_gated_act           h[m, hidden] = act(g) * u
+ *   bsmm_gated_act_backward  dpre = [dh * u * act'(g) | dh * act(g)], laid out like pre; dbias (fp32 [2 * hidden], may be
+ *                            NULL) receives the sums of dpre over the rows, added up in fp32 in a fixed order; it wants
+ *                            `workspace` (bsmm_gated_act_workspace_bytes bytes), else NULL will do
+ *   bsmm_gated_small         h straight from x and the stored fp32 blocks with exact fp32 products: the form for few tokens
+ *                            (the blocks are read once per 8 tokens and nothing else is, weight images and plans included).
+ *                            ptr / idx = CSR of the 2 * hidden-row matrix, bias fp32 [2 * hidden] or NULL
+ * Types: fp32; BSMM_GATED_IO_BF16: h, dh, dpre (and x of bsmm_gated_small) are bf16, pre stays fp32 unless
+ * BSMM_GATED_PRE_BF16 (only together with it); BSMM_GATED_X_BF16: bsmm_gated_small's x is bf16 and h fp32.
+ * All pointers 16-byte aligned (ptr 4, idx 8).
+ */
+#define BSMM_GATED_GELU 0x1u     /* act: GELU (erf form); otherwise SiLU, g / (1 + exp(-g)) */
+#define BSMM_GATED_IO_BF16 0x2u
+#define BSMM_GATED_PRE_BF16 0x4u
+#define BSMM_GATED_X_BF16 0x8u
+int bsmm_gated_act(const void* pre, int64_t m, int64_t hidden, void* h, uint32_t flags, bsmm_stream_t stream);
+int64_t bsmm_gated_act_workspace_bytes(int64_t m, int64_t hidden);
+int bsmm_gated_act_backward(const void* pre, const void* dh, int64_t m, int64_t hidden, void* dpre, float* dbias,
+                            void* workspace, uint32_t flags, bsmm_stream_t stream);
+int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, int64_t nnz,
+                     const float* data, int64_t hidden, const float* bias, void* h, uint32_t flags, bsmm_stream_t stream);
+
+/*
+ * Dropout with the residual add behind it: out[i] = (keep(i) ? x[i] * 65536 / (65536 - cut) : 0) + residual[i] over n
+ * contiguous elements; residual may be NULL.  The mask is never stored: element i draws the (i mod 8)-th 16-bit number (word by
+ * word, low half first) of Philox4x32-10 with key rng[0] and 128-bit counter (i / 8, rng[1]) and is kept when the number is
+ * at least `cut` (0 <= cut < 65536: the rate in units of 2^-16).  The same call on the output's gradient, without residual, is
+ * the backward pass.  x, residual and out have one type, fp32 or bf16 (BSMM_DROPOUT_BF16); out may be x or residual;
+ * 16-byte aligned.  rng: DEVICE int64 [2], read when the kernel runs (a captured call draws anew in every replay if the
+ * graph moves the state on).
+ * bsmm_rng_next: used[0..1] = state[0..1], then state[1] += 1 (both DEVICE int64 [2]): one draw of a state.
+ */
+#define BSMM_DROPOUT_BF16 0x1u
+int bsmm_dropout(const void* x, const void* residual, void* out, int64_t n, uint32_t cut, const int64_t* rng,
+                 uint32_t flags, bsmm_stream_t stream);
+int bsmm_rng_next(int64_t* state, int64_t* used, bsmm_stream_t stream);
+
+/*
+ * Low-rank adapters of many requests: out[t] = base[t] + scaling[a] * (x[t] D_a^T) U_a^T, a = the adapter of the request that
+ * token t belongs to.  Request i owns the tokens offsets[i] <= t < offsets[i + 1] (non-decreasing DEVICE int32 [requests + 1]) and
+ * uses adapter ids[i] (DEVICE int32; a value outside [0, count) means none).  Tokens of no request or no adapter, such as
+ * padding behind the last request, get base[t].
+ *   x [tokens, inner], down [count, rank, inner], up [count, outer, rank]; base (or NULL: zeros) and out [tokens, outer],
+ *   which may be one tensor; all row-major.  inner and outer multiples of 32; rank 16, 32, or a multiple of 64 up to 256
+ *   (smaller ranks are padded with zeros); tokens, requests free.  workspace: bsmm_adapters_workspace_bytes bytes.
+ * Types: fp32; BSMM_ADAPTERS_IN_BF16: x, down and up are bf16; BSMM_ADAPTERS_OUT_BF16 (only together with it): base and out
+ * too.  All sums are fp32; results do not depend on timing.  16-byte aligned (offsets, ids, scaling: 4).
+ */
+#define BSMM_ADAPTERS_IN_BF16 0x1u
+#define BSMM_ADAPTERS_OUT_BF16 0x2u
+int64_t bsmm_adapters_workspace_bytes(int64_t tokens, int64_t inner, int64_t rank);
+int bsmm_adapters(const void* x, int64_t tokens, int64_t inner, int64_t outer, const int32_t* offsets, const int32_t* ids,
+                  int64_t requests, int64_t count, int64_t rank, const void* down, const void* up, const float* scaling,
+                  const void* base, void* out, void* workspace, uint32_t flags, bsmm_stream_t stream);
 
 #ifdef __cplusplus
 }

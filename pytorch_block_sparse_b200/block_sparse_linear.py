@@ -20,6 +20,7 @@ import torch.autograd
 import torch.nn as nn
 
 from . import native
+from .dropout import dropout_residual, new_rng_state, next_rng, rate_units
 from .block_sparse import BlockSparseMatrix, BlockSparseMatrixBase, BlockSparseMatrixEmulator
 
 
@@ -98,9 +99,14 @@ class BlockSparseLinear(nn.Module):
     ``from_dense`` and rescales by ``1/sqrt(density)``.  Square blocks of 32, 64, 96, 128 ... run on the
     tensor-core kernels; other block shapes use the dense-masked emulator class (the reference sends
     everything but 32x32 there).  Parameters live on ``"cuda"``.
+
+    Not in the reference: ``activation`` (``"gelu"``, in the forward kernel's epilogue) and ``dropout``, the rate of a dropout of
+    the output in training mode, before the residual is added; its mask comes from a counter-based generator whose
+    state (a seed from torch's default generator, a counter) lives on the device and is not part of the state dict.
     """
 
     OPTIMIZED_BLOCK_SIZE = 32
+    dropout = 0.0  # layers pickled before there was one
 
     def __init__(
         self,
@@ -112,6 +118,7 @@ class BlockSparseLinear(nn.Module):
         verbose: bool = False,
         block_shape: Tuple[int, int] = (32, 32),
         activation=None,
+        dropout: float = 0.0,
     ):
         super().__init__()
         self.fn = BlockSparseLinearFunction.apply
@@ -120,6 +127,10 @@ class BlockSparseLinear(nn.Module):
         if activation not in (None, "gelu"):
             raise Exception(f"BlockSparseLinear invalid activation={activation}, expected None or 'gelu'")
         self.activation = activation  # not in the reference: applied inside the forward kernel's epilogue
+        if activation is not None and rate_units(dropout) > 0:
+            raise Exception("BlockSparseLinear invalid dropout with an activation: dropout belongs to the output projection")
+        self.dropout = dropout
+        rate_units(dropout)
         # 32x32 blocks and larger square multiples of 32 run on the CUDA kernels (the latter through their
         # 32x32 expansion); every other block shape uses the dense-masked emulator, as in the reference
         self._optimized = (
@@ -160,10 +171,42 @@ class BlockSparseLinear(nn.Module):
                     self.bias.copy_(torch_nn_linear.bias)
         else:
             self.register_parameter("bias", None)
+        if rate_units(dropout) > 0:
+            self.register_buffer("dropout_rng", new_rng_state("cuda"), persistent=False)
 
-    def forward(self, x, residual=None):
+    def forward(self, x, residual=None, adapters=None):
         """``act(x @ W.T + bias + residual)``; ``residual`` (not in the reference) has the output's shape and is
-        added in the kernel's epilogue, like the bias and the layer's ``activation``."""
+        added in the kernel's epilogue, like the bias and the layer's ``activation``.
+
+        With the layer's ``dropout``, in training mode: ``dropout(x @ W.T + bias) + residual``.  ``adapters`` (not in the
+        reference; inference only): a pair of :class:`LowRankAdapters` and :class:`AdapterRequests`, whose product is added
+        to ``x @ W.T`` for the tokens of each request."""
+        if adapters is not None:
+            return self._forward_adapters(x, residual, *adapters)
+        if self.training and self.dropout > 0:
+            return self._dropped(self._project(x), residual)
+        return self._project(x, residual)
+
+    def _dropped(self, y, residual):
+        if rate_units(self.dropout) == 0:
+            return y if residual is None else y + residual
+        if residual is not None:
+            wide = torch.promote_types(y.dtype, residual.dtype)
+            y, residual = y.to(wide), residual.to(wide).expand_as(y)
+        return dropout_residual(y, self.dropout, next_rng(self.dropout_rng), residual=residual)
+
+    def _forward_adapters(self, x, residual, adapters, requests):
+        if adapters.in_features != self.in_features or adapters.out_features != self.out_features:
+            raise Exception("adapters of %d -> %d features beside a layer of %d -> %d" % (
+                adapters.in_features, adapters.out_features, self.in_features, self.out_features))
+        drop = self.training and self.dropout > 0
+        if self.activation is not None:
+            # the activation sits in the projection's epilogue: what the adapters add goes in with the residual
+            return self._project(x, adapters(x, requests, base=residual.float() if residual is not None else None, dtype=torch.float32))
+        y = adapters(x, requests, base=self._project(x, None if drop else residual), inplace=True)
+        return self._dropped(y, residual) if drop else y
+
+    def _project(self, x, residual=None):
         if self._optimized:
             if residual is None and self.activation is None:
                 return self.fn(x, self.weight.get_differentiable_data(), self.weight, self.bias)

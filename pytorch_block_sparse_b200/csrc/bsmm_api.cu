@@ -21,6 +21,11 @@ void forget_earlier_errors() { (void)cudaGetLastError(); }
 
 }  // namespace
 
+namespace bsmm {
+// for the entry points of other translation units (bsmm_feedforward_api.cu)
+int report_cuda(cudaError_t err) { return cuda_status(err); }
+}  // namespace bsmm
+
 extern "C" {
 
 int bsmm_abi_version(void) { return BSMM_ABI_VERSION; }

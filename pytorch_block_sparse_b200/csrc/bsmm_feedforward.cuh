@@ -1,0 +1,98 @@
+// Shared declarations of the operators around a block-sparse projection: the gated feed-forward block, dropout with the
+// residual add, and low-rank adapters.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "bsmm_common.cuh"
+
+namespace bsmm {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// eight consecutive values, 16-byte aligned
+__device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(u[j] << 16);
+        v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+    }
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float low, float high) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    unpack8(*reinterpret_cast<const uint4*>(p), v);
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+// The gate's activation, in fp32.  kind: 0 SiLU g / (1 + exp(-g)), 1 GELU (erf form).
+__device__ __forceinline__ float gate_act(float g, int kind) {
+    if (kind == 0) return g / (1.f + expf(-g));
+    return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+}
+// value and derivative
+__device__ __forceinline__ void gate_act_grad(float g, int kind, float& value, float& slope) {
+    if (kind == 0) {
+        const float s = 1.f / (1.f + expf(-g));
+        value = g * s;
+        slope = s * (1.f + g * (1.f - s));
+    } else {
+        const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+        value = g * cdf;
+        slope = cdf + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+    }
+}
+
+// launchers
+cudaError_t launch_dropout(const void* x, const void* residual, void* out, int64_t n, uint32_t cut, const int64_t* rng,
+                           bool bf16, cudaStream_t stream);
+cudaError_t launch_rng_next(int64_t* state, int64_t* used, cudaStream_t stream);
+
+cudaError_t launch_gated_act(const void* pre, int64_t m, int64_t hidden, void* h, int act, bool pre_bf16, bool io_bf16,
+                             cudaStream_t stream);
+int64_t gated_act_workspace_bytes(int64_t m, int64_t hidden);
+cudaError_t launch_gated_act_backward(const void* pre, const void* dh, int64_t m, int64_t hidden, void* dpre,
+                                      float* dbias, float* workspace, int act, bool pre_bf16, bool io_bf16,
+                                      cudaStream_t stream);
+cudaError_t launch_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx,
+                               const float* data, int64_t hidden, const float* bias, void* h, int act, bool x_bf16,
+                               bool h_bf16, cudaStream_t stream);
+
+struct AdapterCall {
+    const void* x;           // [tokens, inner]
+    const void* down;        // [count, rank, inner], rank padded to a multiple of 16 with zero rows
+    const void* up;          // [count, outer, rank]
+    const float* scaling;    // [count]
+    const int32_t* offsets;  // [requests + 1]
+    const int32_t* ids;      // [requests]
+    const void* base;        // [tokens, outer] or null (zeros); may be `out`
+    void* out;               // [tokens, outer]
+    float* workspace;
+    int64_t tokens, inner, outer, requests, count, rank;
+};
+int64_t adapters_workspace_bytes(int64_t tokens, int64_t inner, int64_t rank);
+// in_bf16: x, down and up; out_bf16: base and out
+cudaError_t launch_adapters(const AdapterCall& call, bool in_bf16, bool out_bf16, cudaStream_t stream);
+
+}  // namespace bsmm

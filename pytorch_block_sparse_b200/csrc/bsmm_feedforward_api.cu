@@ -1,0 +1,122 @@
+// extern "C" entry points of the operators around a block-sparse projection: argument validation and launches.
+#include "bsmm_feedforward.cuh"
+
+namespace bsmm {
+int report_cuda(cudaError_t err);  // bsmm_api.cu: status code, and the error bsmm_last_cuda_error returns
+}
+
+namespace {
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// rows x cols elements of at most 4 bytes stay addressable, and every product of sizes below fits 63 bits
+bool too_large(int64_t rows, int64_t cols) { return rows > 0x7fffffffll || cols > 0x7fffffffll || (cols > 0 && rows > (1ll << 40) / cols); }
+
+int gated_types(uint32_t flags) {
+    if ((flags & ~(BSMM_GATED_GELU | BSMM_GATED_IO_BF16 | BSMM_GATED_PRE_BF16 | BSMM_GATED_X_BF16)) != 0) return BSMM_ERR_UNSUPPORTED;
+    if ((flags & BSMM_GATED_PRE_BF16) != 0 && (flags & BSMM_GATED_IO_BF16) == 0) return BSMM_ERR_UNSUPPORTED;
+    return BSMM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bsmm_gated_act(const void* pre, int64_t m, int64_t hidden, void* h, uint32_t flags, bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (m < 0 || hidden < 0 || (hidden % 32) != 0) return BSMM_ERR_INVALID_ARGUMENT;
+    const int status = gated_types(flags);
+    if (status != BSMM_OK || (flags & BSMM_GATED_X_BF16) != 0) return BSMM_ERR_UNSUPPORTED;
+    if (m == 0 || hidden == 0) return BSMM_OK;
+    if (pre == nullptr || h == nullptr || !aligned(pre, 16) || !aligned(h, 16)) return BSMM_ERR_INVALID_ARGUMENT;
+    if (too_large(m, 2 * hidden)) return BSMM_ERR_TOO_LARGE;
+    return bsmm::report_cuda(bsmm::launch_gated_act(pre, m, hidden, h, (flags & BSMM_GATED_GELU) != 0,
+                                                    (flags & BSMM_GATED_PRE_BF16) != 0, (flags & BSMM_GATED_IO_BF16) != 0,
+                                                    static_cast<cudaStream_t>(stream)));
+}
+
+int64_t bsmm_gated_act_workspace_bytes(int64_t m, int64_t hidden) {
+    if (m < 0 || hidden < 0 || too_large(m, 2 * hidden)) return -1;
+    return bsmm::gated_act_workspace_bytes(m, hidden);
+}
+
+int bsmm_gated_act_backward(const void* pre, const void* dh, int64_t m, int64_t hidden, void* dpre, float* dbias,
+                            void* workspace, uint32_t flags, bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (m < 0 || hidden < 0 || (hidden % 32) != 0) return BSMM_ERR_INVALID_ARGUMENT;
+    const int status = gated_types(flags);
+    if (status != BSMM_OK || (flags & BSMM_GATED_X_BF16) != 0) return BSMM_ERR_UNSUPPORTED;
+    if (hidden == 0) return BSMM_OK;
+    if (m > 0 && (pre == nullptr || dh == nullptr || dpre == nullptr || (dbias != nullptr && workspace == nullptr)))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (!aligned(pre, 16) || !aligned(dh, 16) || !aligned(dpre, 16) || !aligned(dbias, 4) || !aligned(workspace, 16))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (too_large(m, 2 * hidden)) return BSMM_ERR_TOO_LARGE;
+    return bsmm::report_cuda(bsmm::launch_gated_act_backward(
+        pre, dh, m, hidden, dpre, dbias, static_cast<float*>(workspace), (flags & BSMM_GATED_GELU) != 0,
+        (flags & BSMM_GATED_PRE_BF16) != 0, (flags & BSMM_GATED_IO_BF16) != 0, static_cast<cudaStream_t>(stream)));
+}
+
+int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, int64_t nnz,
+                     const float* data, int64_t hidden, const float* bias, void* h, uint32_t flags, bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (m < 0 || k < 0 || hidden < 0 || nnz < 0 || (hidden % 32) != 0 || (k % 32) != 0) return BSMM_ERR_INVALID_ARGUMENT;
+    if (gated_types(flags) != BSMM_OK || (flags & BSMM_GATED_PRE_BF16) != 0) return BSMM_ERR_UNSUPPORTED;
+    if (m == 0 || hidden == 0) return BSMM_OK;
+    if (ptr == nullptr || h == nullptr || (nnz > 0 && (x == nullptr || idx == nullptr || data == nullptr)))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (!aligned(x, 16) || !aligned(ptr, 4) || !aligned(idx, 8) || !aligned(data, 16) || !aligned(bias, 4) || !aligned(h, 16))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (nnz > 0x7fffffff || too_large(m, k) || too_large(m, hidden) || (m + 7) / 8 > 65535) return BSMM_ERR_TOO_LARGE;
+    const bool io16 = (flags & BSMM_GATED_IO_BF16) != 0;
+    return bsmm::report_cuda(bsmm::launch_gated_small(x, m, k, ptr, idx, data, hidden, bias, h, (flags & BSMM_GATED_GELU) != 0,
+                                                      io16 || (flags & BSMM_GATED_X_BF16) != 0, io16,
+                                                      static_cast<cudaStream_t>(stream)));
+}
+
+int bsmm_dropout(const void* x, const void* residual, void* out, int64_t n, uint32_t cut, const int64_t* rng,
+                 uint32_t flags, bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (n < 0 || cut >= 65536u) return BSMM_ERR_INVALID_ARGUMENT;
+    if ((flags & ~BSMM_DROPOUT_BF16) != 0) return BSMM_ERR_UNSUPPORTED;
+    if (n == 0) return BSMM_OK;
+    if (x == nullptr || out == nullptr || rng == nullptr) return BSMM_ERR_INVALID_ARGUMENT;
+    if (!aligned(x, 16) || !aligned(residual, 16) || !aligned(out, 16) || !aligned(rng, 8)) return BSMM_ERR_INVALID_ARGUMENT;
+    return bsmm::report_cuda(bsmm::launch_dropout(x, residual, out, n, cut, rng, (flags & BSMM_DROPOUT_BF16) != 0,
+                                                  static_cast<cudaStream_t>(stream)));
+}
+
+int bsmm_rng_next(int64_t* state, int64_t* used, bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (state == nullptr || used == nullptr || !aligned(state, 8) || !aligned(used, 8)) return BSMM_ERR_INVALID_ARGUMENT;
+    return bsmm::report_cuda(bsmm::launch_rng_next(state, used, static_cast<cudaStream_t>(stream)));
+}
+
+int64_t bsmm_adapters_workspace_bytes(int64_t tokens, int64_t inner, int64_t rank) {
+    if (tokens < 0 || inner < 0 || (inner % 32) != 0 || rank < 0 || rank > 256 || too_large(tokens, inner)) return -1;
+    return inner == 0 ? 0 : bsmm::adapters_workspace_bytes(tokens, inner, rank);
+}
+
+int bsmm_adapters(const void* x, int64_t tokens, int64_t inner, int64_t outer, const int32_t* offsets, const int32_t* ids,
+                  int64_t requests, int64_t count, int64_t rank, const void* down, const void* up, const float* scaling,
+                  const void* base, void* out, void* workspace, uint32_t flags, bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (tokens < 0 || inner <= 0 || outer < 0 || requests < 0 || count < 0 || (inner % 32) != 0 || (outer % 32) != 0)
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (rank != 16 && rank != 32 && (rank <= 0 || rank > 256 || (rank % 64) != 0)) return BSMM_ERR_INVALID_ARGUMENT;
+    if ((flags & ~(BSMM_ADAPTERS_IN_BF16 | BSMM_ADAPTERS_OUT_BF16)) != 0 || flags == BSMM_ADAPTERS_OUT_BF16) return BSMM_ERR_UNSUPPORTED;
+    if (tokens == 0 || outer == 0) return BSMM_OK;
+    if (x == nullptr || offsets == nullptr || out == nullptr || workspace == nullptr || (requests > 0 && ids == nullptr) ||
+        (count > 0 && (down == nullptr || up == nullptr || scaling == nullptr)))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (!aligned(x, 16) || !aligned(offsets, 4) || !aligned(ids, 4) || !aligned(down, 16) || !aligned(up, 16) ||
+        !aligned(scaling, 4) || !aligned(base, 16) || !aligned(out, 16) || !aligned(workspace, 16))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (too_large(tokens, inner) || too_large(tokens, outer) || requests > 0x7ffffffell || count > 0x7fffffffll) return BSMM_ERR_TOO_LARGE;
+    bsmm::AdapterCall call = {x, down, up, scaling, offsets, ids, base, out, static_cast<float*>(workspace),
+                              tokens, inner, outer, requests, count, rank};
+    return bsmm::report_cuda(bsmm::launch_adapters(call, (flags & BSMM_ADAPTERS_IN_BF16) != 0,
+                                                   (flags & BSMM_ADAPTERS_OUT_BF16) != 0, static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

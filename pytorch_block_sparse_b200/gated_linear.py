@@ -1,0 +1,180 @@
+"""The gated feed-forward block on block-sparse weights: ``h = act(x @ Wg.T + bg) * (x @ Wu.T + bu)``.
+
+Both projections live in ONE :class:`BlockSparseMatrix` of ``2 * hidden`` rows whose block-rows alternate -- block-row ``2j`` is
+the gate's block-row ``j``, ``2j + 1`` the up projection's -- so that one product computes both, the two halves of a hidden unit
+meet in the same tile, and each gradient is one product too.  The pattern, the sparsity optimizer and checkpoints see
+an ordinary block-sparse matrix.  The reference has no gated layer: its user builds two ``BlockSparseLinear`` and multiplies
+(``block_sparse_linear.py:157-233`` is the layer this one stands beside).
+"""
+import math
+
+import numpy
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import native
+from .block_sparse import BlockSparseMatrix
+
+# Up to this many tokens inference computes from the stored blocks directly (``bsmm_gated_small``).
+SMALL_TOKENS = 32
+
+
+def interleave_rows(gate, up):
+    """``[hidden, ...]`` of the gate and of the up projection -> ``[2 * hidden, ...]``, 32 rows of each in turn."""
+    tail = gate.shape[1:]
+    return torch.stack([gate.reshape(-1, 32, *tail), up.reshape(-1, 32, *tail)], 1).reshape(-1, *tail)
+
+
+def split_rows(both):
+    """Inverse of :func:`interleave_rows`: ``(gate, up)``."""
+    tail = both.shape[1:]
+    parts = both.reshape(-1, 2, 32, *tail)
+    return parts[:, 0].reshape(-1, *tail), parts[:, 1].reshape(-1, *tail)
+
+
+class BlockSparseGatedFunction(torch.autograd.Function):
+    """``apply(input, weight_data, weight, bias, activation, precision)`` with ``input [m, k]``."""
+
+    @staticmethod
+    def forward(ctx, input, weight_data, weight, bias, activation, precision):
+        ctx.weight, ctx.activation, ctx.precision = weight, activation, precision
+        # packed once per forward, never cached: writes through ``.data`` do not bump version counters; backward uses the
+        # weights that the forward saw
+        ctx.packed = weight.packed_weights(precision)
+        out_dtype = _out_dtype(input, precision)
+        pre = weight.reverse_matmul(input.float(), transpose=True, bias=bias, packed=ctx.packed)
+        h = native.gated_act(pre, activation, out_dtype)
+        ctx.save_for_backward(input, pre)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        input, pre = ctx.saved_tensors
+        weight = ctx.weight
+        dpre, dbias = native.gated_act_backward(pre, grad.contiguous(), ctx.activation, ctx.needs_input_grad[3])
+        grad_weight = grad_input = None
+        # the weight gradient first, as in BlockSparseLinearFunction: its all-reduce can overlap the input gradient
+        if ctx.needs_input_grad[1]:
+            grad_weight = weight.matmul_with_output_sparse_support(dpre, input, precision=ctx.precision)
+        if ctx.needs_input_grad[0]:
+            grad_input = weight.reverse_matmul(dpre, transpose=False, packed=ctx.packed).to(input.dtype)
+        return grad_input, grad_weight, None, dbias, None, None
+
+
+def _out_dtype(x, precision):
+    """bf16 tensors stay bf16 in the 'bf16' precision; every other combination computes fp32 (as BlockSparseLinear)."""
+    name = native.default_precision() if precision is None else precision
+    return torch.bfloat16 if x.dtype == torch.bfloat16 and name == "bf16" else torch.float32
+
+
+class BlockSparseGatedLinear(nn.Module):
+    """``act(gate(x)) * up(x)`` with block-sparse projections ``in_features -> hidden_features`` (multiples of 32).
+
+    ``density``: share of the 32x32 blocks stored, ``int(density * in * hidden / 1024)`` positions drawn at random, the same for
+    both projections (a hidden block reads the same inputs through both).  ``weight`` hands in the matrix instead,
+    ``[2 * hidden, in]`` with alternating block-rows and any pattern.  ``activation``: ``"silu"`` or ``"gelu"`` (erf form).
+    ``bias``: fp32 ``[2 * hidden]``, laid out like the weight's rows.  ``precision``: as ``set_default_precision``; ``None`` follows the
+    default at each call.  Input: fp32 or bf16 ``[..., in]``; the output is bf16 for bf16 input in the ``"bf16"`` precision, else
+    fp32.  Without gradients and up to ``SMALL_TOKENS`` tokens the products are exact fp32 in every precision."""
+
+    def __init__(self, in_features, hidden_features, bias=True, density=0.5, activation="silu", weight=None, precision=None):
+        super().__init__()
+        if in_features <= 0 or in_features % 32 != 0:
+            raise Exception(f"BlockSparseGatedLinear invalid in_features={in_features}, should be multiple of 32")
+        if hidden_features <= 0 or hidden_features % 32 != 0:
+            raise Exception(f"BlockSparseGatedLinear invalid hidden_features={hidden_features}, should be multiple of 32")
+        if activation not in ("silu", "gelu"):
+            raise Exception(f"BlockSparseGatedLinear invalid activation={activation}, expected 'silu' or 'gelu'")
+        if precision is not None and precision not in native.PRECISIONS:
+            raise ValueError("unknown precision %r, expected one of %s" % (precision, sorted(native.PRECISIONS)))
+        self.in_features, self.hidden_features = in_features, hidden_features
+        self.activation, self.precision = activation, precision
+        if weight is None:
+            if density < 0 or density > 1:
+                raise Exception(f"BlockSparseGatedLinear invalid density={density}")
+            rows, cols = hidden_features // 32, in_features // 32
+            cells = numpy.random.choice(rows * cols, size=int(density * rows * cols), replace=False)
+            weight = self._matrix(cells, rows, cols, "cuda")
+            with torch.no_grad():
+                weight.data.normal_()
+        elif not isinstance(weight, BlockSparseMatrix) or tuple(weight.block_shape) != (32, 32):
+            raise Exception("BlockSparseGatedLinear weight should be a BlockSparseMatrix with 32x32 blocks")
+        elif tuple(weight.shape) != (2 * hidden_features, in_features):
+            raise Exception("BlockSparseGatedLinear weight should be of shape (%d, %d), not %s" % (
+                2 * hidden_features, in_features, tuple(weight.shape)))
+        self.weight = weight
+        if bias:
+            self.bias = nn.Parameter(torch.zeros(2 * hidden_features, device=weight.data.device))
+        else:
+            self.register_parameter("bias", None)
+
+    @staticmethod
+    def _matrix(cells, rows, cols, device):
+        """Matrix of zeros with both projections' blocks at the positions ``cells`` of the ``rows`` x ``cols`` grid."""
+        mask = torch.zeros(rows * cols, dtype=torch.bool, device=device)
+        mask[torch.as_tensor(cells, dtype=torch.int64, device=device)] = True
+        mask = mask.view(rows, cols).repeat_interleave(2, 0)
+        data = torch.zeros((2 * len(cells) * 32, 32), dtype=torch.float32, device=device)
+        return BlockSparseMatrix((2 * rows * 32, cols * 32), mask, data)
+
+    @classmethod
+    def from_linears(cls, gate, up, density=1.0, activation="silu", precision=None):
+        """From two dense ``nn.Linear`` of one shape: ``density`` of their blocks, drawn at random, scaled by
+        ``1 / sqrt(density)`` as ``BlockSparseLinear`` does."""
+        if gate.weight.shape != up.weight.shape or (gate.bias is None) != (up.bias is None):
+            raise Exception("gate and up should be two linear layers of one shape, both with a bias or both without")
+        hidden, inner = gate.weight.shape
+        if hidden % 32 != 0 or inner % 32 != 0:
+            raise Exception(f"BlockSparseGatedLinear invalid layer {hidden}x{inner}, should be multiples of 32")
+        if density <= 0 or density > 1:
+            raise Exception(f"BlockSparseGatedLinear invalid density={density}")
+        rows, cols = hidden // 32, inner // 32
+        cells = numpy.random.choice(rows * cols, size=int(density * rows * cols), replace=False)
+        with torch.no_grad():
+            weight = cls._matrix(cells, rows, cols, "cuda")
+            BlockSparseMatrix.from_dense(interleave_rows(gate.weight.detach().float().cuda(), up.weight.detach().float().cuda()),
+                                         out=weight)
+            weight.multiply_(1.0 / math.sqrt(density))
+            layer = cls(inner, hidden, bias=gate.bias is not None, activation=activation, weight=weight, precision=precision)
+            if gate.bias is not None:
+                layer.bias.copy_(interleave_rows(gate.bias.detach().float().cuda(), up.bias.detach().float().cuda()))
+        return layer
+
+    def to_dense(self):
+        """``(gate, up)``: the two weights as dense ``[hidden, in]`` matrices."""
+        return split_rows(self.weight.to_dense())
+
+    def forward(self, x):
+        if x.dim() < 2:
+            raise Exception(f"Invalid dimensions for x {tuple(x.shape)} : x should have at least 2 dimensions.")
+        if x.shape[-1] != self.in_features:
+            raise Exception("Invalid matrices sizes (%d, %d) x (%d, %d)" % (
+                x.numel() // max(1, x.shape[-1]), x.shape[-1], self.in_features, 2 * self.hidden_features))
+        if x.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("BlockSparseGatedLinear takes float32 or bfloat16 tensors, got %s" % x.dtype)
+        self.weight._require_cuda()
+        if x.device != self.weight.data.device:
+            raise native.NativeError("x is on %s, the layer on %s" % (x.device, self.weight.data.device))
+        lead = x.shape[:-1]
+        flat = x.reshape(-1, self.in_features).contiguous()
+        data = self.weight.get_differentiable_data()
+        if torch.is_grad_enabled() and (x.requires_grad or data.requires_grad or (self.bias is not None and self.bias.requires_grad)):
+            h = BlockSparseGatedFunction.apply(flat, data, self.weight, self.bias, self.activation, self.precision)
+        else:
+            h = self._infer(flat)
+        return h.reshape(*lead, self.hidden_features)
+
+    def _infer(self, flat):
+        weight, bias = self.weight, self.bias.detach() if self.bias is not None else None
+        out_dtype = _out_dtype(flat, self.precision)
+        if flat.shape[0] <= SMALL_TOKENS:
+            return native.gated_small(flat, weight.row_start_ends_a, weight.cols_a, weight.data, self.hidden_features, bias,
+                                      self.activation, out_dtype)
+        pre = weight.reverse_matmul(flat.float(), transpose=True, bias=bias, precision=self.precision)
+        return native.gated_act(pre, self.activation, out_dtype)
+
+    def extra_repr(self):
+        return "in_features={}, hidden_features={}, bias={}, activation={}, block_count={}".format(
+            self.in_features, self.hidden_features, self.bias is not None, self.activation, self.weight.blocks.shape[0] // 2)

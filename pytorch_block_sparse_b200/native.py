@@ -13,11 +13,14 @@ _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libbsmm_b200.so")
 
 # mirrors include/bsmm_b200.h
-ABI_VERSION = 2
+ABI_VERSION = 3
 OK = 0
 PREC_FP32_SIMT, PREC_TF32X3, PREC_BF16, PREC_TF32, PREC_BF16X3 = 0, 1, 2, 3, 4
 DSD_DGRAD, DSD_OUT_COLMAJOR, DSD_GELU, DSD_IO_BF16 = 0x10, 0x20, 0x40, 0x80
 SDDMM_A_COLMAJOR, SDDMM_B_COLMAJOR, SDDMM_IO_BF16 = 0x10, 0x20, 0x40
+GATED_GELU, GATED_IO_BF16, GATED_PRE_BF16, GATED_X_BF16 = 0x1, 0x2, 0x4, 0x8
+DROPOUT_BF16 = 0x1
+ADAPTERS_IN_BF16, ADAPTERS_OUT_BF16 = 0x1, 0x2
 
 PRECISIONS = {"fp32": PREC_FP32_SIMT, "simt": PREC_FP32_SIMT, "tf32x3": PREC_TF32X3, "tf32": PREC_TF32, "bf16": PREC_BF16,
               "bf16x3": PREC_BF16X3}
@@ -47,6 +50,14 @@ EXPORTS = (
     "bsmm_select_lowest",
     "bsmm_sample_free_cells",
     "bsmm_move_blocks",
+    "bsmm_gated_act",
+    "bsmm_gated_act_workspace_bytes",
+    "bsmm_gated_act_backward",
+    "bsmm_gated_small",
+    "bsmm_dropout",
+    "bsmm_rng_next",
+    "bsmm_adapters_workspace_bytes",
+    "bsmm_adapters",
 )
 
 _lib = None
@@ -120,6 +131,22 @@ def load():
     lib.bsmm_sample_free_cells.argtypes = [vp, i64, i64, i64, c.c_uint64, vp, vp, vp, vp]
     lib.bsmm_move_blocks.restype = i32
     lib.bsmm_move_blocks.argtypes = [vp, vp, vp, i64, i64, i64, vp, vp]
+    lib.bsmm_gated_act.restype = i32
+    lib.bsmm_gated_act.argtypes = [vp, i64, i64, vp, u32, vp]
+    lib.bsmm_gated_act_workspace_bytes.restype = i64
+    lib.bsmm_gated_act_workspace_bytes.argtypes = [i64, i64]
+    lib.bsmm_gated_act_backward.restype = i32
+    lib.bsmm_gated_act_backward.argtypes = [vp, vp, i64, i64, vp, vp, vp, u32, vp]
+    lib.bsmm_gated_small.restype = i32
+    lib.bsmm_gated_small.argtypes = [vp, i64, i64, vp, vp, i64, vp, i64, vp, vp, u32, vp]
+    lib.bsmm_dropout.restype = i32
+    lib.bsmm_dropout.argtypes = [vp, vp, vp, i64, u32, vp, u32, vp]
+    lib.bsmm_rng_next.restype = i32
+    lib.bsmm_rng_next.argtypes = [vp, vp, vp]
+    lib.bsmm_adapters_workspace_bytes.restype = i64
+    lib.bsmm_adapters_workspace_bytes.argtypes = [i64, i64, i64]
+    lib.bsmm_adapters.restype = i32
+    lib.bsmm_adapters.argtypes = [vp, i64, i64, i64, vp, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, u32, vp]
     if lib.bsmm_abi_version() != ABI_VERSION:
         raise NativeError("libbsmm_b200.so has ABI %d, this package expects %d" % (lib.bsmm_abi_version(), ABI_VERSION))
     _lib = lib
@@ -532,5 +559,107 @@ def sddmm(a, a_rowmajor, b, b_rowmajor, blocks, out, precision=None, block_sumsq
                 _ptr(block_sumsq), _ptr(ws), flags, _stream(a.device),
             ),
             "bsmm_sddmm",
+        )
+    return out
+
+
+def _gated_flags(activation):
+    if activation not in ("silu", "gelu"):
+        raise ValueError("unknown gate activation %r ('silu' or 'gelu')" % (activation,))
+    return GATED_GELU if activation == "gelu" else 0
+
+
+def gated_act(pre, activation, out_dtype):
+    """``act(g) * u`` of pre-activations ``[m, 2 * hidden]`` whose columns alternate in blocks of 32, g then u
+    (``bsmm_gated_act``)."""
+    _need_cuda(pre, "pre")
+    m, hidden = pre.shape[0], pre.shape[1] // 2
+    out = torch.empty((m, hidden), dtype=out_dtype, device=pre.device)
+    flags = _gated_flags(activation) | (GATED_IO_BF16 if out_dtype == torch.bfloat16 else 0)
+    flags |= GATED_PRE_BF16 if pre.dtype == torch.bfloat16 else 0
+    with torch.cuda.device(pre.device):
+        check(load().bsmm_gated_act(_ptr(pre), m, hidden, _ptr(out), flags, _stream(pre.device)), "bsmm_gated_act")
+    return out
+
+
+def gated_act_backward(pre, dh, activation, want_bias):
+    """``(dpre, dbias)`` of :func:`gated_act`: ``dpre`` like ``pre`` in ``dh``'s type, ``dbias`` its fp32 sum over the rows
+    (``None`` unless wanted)."""
+    _need_cuda(pre, "pre")
+    lib = load()
+    m, hidden = dh.shape
+    dpre = torch.empty(pre.shape, dtype=dh.dtype, device=pre.device)
+    dbias = ws = None
+    if want_bias:
+        dbias = torch.empty(2 * hidden, dtype=torch.float32, device=pre.device)
+        ws = torch.empty(max(16, lib.bsmm_gated_act_workspace_bytes(m, hidden)), dtype=torch.uint8, device=pre.device)
+    flags = _gated_flags(activation) | (GATED_IO_BF16 if dh.dtype == torch.bfloat16 else 0)
+    flags |= GATED_PRE_BF16 if pre.dtype == torch.bfloat16 else 0
+    with torch.cuda.device(pre.device):
+        check(
+            lib.bsmm_gated_act_backward(_ptr(pre), _ptr(_aligned(dh)), m, hidden, _ptr(dpre), _ptr(dbias), _ptr(ws), flags,
+                                        _stream(pre.device)),
+            "bsmm_gated_act_backward",
+        )
+    return dpre, dbias
+
+
+def gated_small(x, ptr, idx, data, hidden, bias, activation, out_dtype):
+    """The gated block for few tokens (``bsmm_gated_small``): ``x`` contiguous ``[m, k]``, ``ptr`` / ``idx`` / ``data`` the CSR
+    buffers and blocks of the ``2 * hidden``-row matrix."""
+    _need_cuda(x, "x")
+    m, k = x.shape
+    out = torch.empty((m, hidden), dtype=out_dtype, device=x.device)
+    flags = _gated_flags(activation)
+    if x.dtype == torch.bfloat16:
+        flags |= GATED_IO_BF16 if out_dtype == torch.bfloat16 else GATED_X_BF16
+    x, ptr, idx, data, bias = _aligned(x), _aligned(ptr), _aligned(idx), _aligned(data.detach()), _aligned(bias)
+    with torch.cuda.device(x.device):
+        check(
+            load().bsmm_gated_small(_ptr(x), m, k, _ptr(ptr), _ptr(idx), idx.shape[0], _ptr(data), hidden, _ptr(bias),
+                                    _ptr(out), flags, _stream(x.device)),
+            "bsmm_gated_small",
+        )
+    return out
+
+
+def dropout(x, residual, cut, rng):
+    """``dropout(x) + residual`` by the mask of ``rng`` (int64 ``[2]``: seed, counter) at rate ``cut / 65536`` (``bsmm_dropout``);
+    contiguous tensors of one type."""
+    _need_cuda(x, "x")
+    x = _aligned(x)
+    residual = _aligned(residual)
+    out = torch.empty_like(x)
+    flags = DROPOUT_BF16 if x.dtype == torch.bfloat16 else 0
+    with torch.cuda.device(x.device):
+        check(load().bsmm_dropout(_ptr(x), _ptr(residual), _ptr(out), x.numel(), cut, _ptr(rng), flags, _stream(x.device)),
+              "bsmm_dropout")
+    return out
+
+
+def rng_next(state):
+    """The (seed, counter) to draw with now, as a new int64 ``[2]`` tensor; the state's counter moves on (``bsmm_rng_next``)."""
+    _need_cuda(state, "state")
+    used = torch.empty(2, dtype=torch.int64, device=state.device)
+    with torch.cuda.device(state.device):
+        check(load().bsmm_rng_next(_ptr(state), _ptr(used), _stream(state.device)), "bsmm_rng_next")
+    return used
+
+
+def adapters(x, offsets, ids, down, up, scaling, base, out):
+    """``out = base + scaling[a] * (x @ down[a].T) @ up[a].T`` for each token's adapter ``a`` (``bsmm_adapters``); ``out`` may be
+    ``base``; all contiguous."""
+    _need_cuda(x, "x")
+    lib = load()
+    tokens, inner = x.shape
+    count, rank = down.shape[0], down.shape[1]
+    x = _aligned(x)
+    ws = torch.empty(max(16, lib.bsmm_adapters_workspace_bytes(tokens, inner, rank)), dtype=torch.uint8, device=x.device)
+    flags = (ADAPTERS_IN_BF16 if x.dtype == torch.bfloat16 else 0) | (ADAPTERS_OUT_BF16 if out.dtype == torch.bfloat16 else 0)
+    with torch.cuda.device(x.device):
+        check(
+            lib.bsmm_adapters(_ptr(x), tokens, inner, up.shape[1], _ptr(offsets), _ptr(ids), ids.shape[0], count, rank,
+                              _ptr(down), _ptr(up), _ptr(scaling), _ptr(base), _ptr(out), _ptr(ws), flags, _stream(x.device)),
+            "bsmm_adapters",
         )
     return out
