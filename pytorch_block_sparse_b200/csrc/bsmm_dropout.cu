@@ -38,38 +38,52 @@ __device__ __forceinline__ float dropped(float x, uint32_t number, uint32_t cut,
     return number >= cut ? x * scale : 0.f;  // a selection: a dropped infinity or NaN leaves nothing behind
 }
 
+// A thread takes kGroups groups, 256 apart, and asks for all of them before it draws: with one group per thread too little
+// is in flight, and the ~110 integer instructions of a group come on top of the memory's latency instead of under it
+// (16384 x 4096 bf16 values without residual, 268 MB: KGROUPS_NOTE).
 // Whole groups move with 16-byte accesses (the caller aligns the pointers), the ragged last one value by value.
-template <typename T, bool kResidual>
+template <typename T, bool kResidual, int kGroups>
 __global__ void __launch_bounds__(256)
 dropout_kernel(const T* __restrict__ x, const T* residual, T* out, int64_t n, uint32_t cut, float scale,
                const int64_t* __restrict__ rng) {
+    const int64_t whole = n / 8, g0 = (int64_t)blockIdx.x * (256 * kGroups) + threadIdx.x;
+    Raw8<T> v[kGroups], r[kResidual ? kGroups : 1];
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+        const int64_t g = g0 + j * 256;
+        if (g < whole) {
+            v[j].load(x + g * 8);
+            if (kResidual) r[j].load(residual + g * 8);
+        }
+    }
     const uint64_t seed = (uint64_t)rng[0], counter = (uint64_t)rng[1];
-    const int64_t groups = (n + 7) / 8;
-    for (int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t i0 = g * 8;
-        float v[8], r[8];
-        if (i0 + 8 <= n) {
-            load8(x + i0, v);
-            if (kResidual) load8(residual + i0, r);
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) {
+        const int64_t g = g0 + j * 256, i0 = g * 8;
+        if (i0 >= n) break;
+        const Philox w = philox4x32((uint64_t)g, counter, seed);
+        float f[8], add[8];
+        if (g < whole) {
+            v[j].unpack(f);
+            if (kResidual) r[j].unpack(add);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = i0 + j < n ? to_float(x[i0 + j]) : 0.f;
-                if (kResidual) r[j] = i0 + j < n ? to_float(residual[i0 + j]) : 0.f;
+            for (int e = 0; e < 8; ++e) {
+                f[e] = i0 + e < n ? to_float(x[i0 + e]) : 0.f;
+                if (kResidual) add[e] = i0 + e < n ? to_float(residual[i0 + e]) : 0.f;
             }
         }
-        const Philox w = philox4x32((uint64_t)g, counter, seed);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = dropped(v[j], (w.v[j >> 1] >> ((j & 1) * 16)) & 0xFFFFu, cut, scale);
-            if (kResidual) v[j] += r[j];
+        for (int e = 0; e < 8; ++e) {
+            f[e] = dropped(f[e], (e & 1) ? w.v[e >> 1] >> 16 : w.v[e >> 1] & 0xFFFFu, cut, scale);
+            if (kResidual) f[e] += add[e];
         }
-        if (i0 + 8 <= n) {
-            store8(out + i0, v);
+        if (g < whole) {
+            store8(out + i0, f);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (i0 + j < n) out[i0 + j] = from_float<T>(v[j]);
+            for (int e = 0; e < 8; ++e)
+                if (i0 + e < n) out[i0 + e] = from_float<T>(f[e]);
         }
     }
 }
@@ -86,14 +100,21 @@ cudaError_t launch(const void* x, const void* residual, void* out, int64_t n, ui
                    cudaStream_t stream) {
     const float scale = 65536.f / (float)(65536u - cut);
     const int64_t groups = (n + 7) / 8;
-    const int64_t blocks = (groups + 255) / 256;
-    const unsigned grid = (unsigned)(blocks < (1ll << 30) ? blocks : (1ll << 30));
-    if (residual != nullptr)
-        dropout_kernel<T, true><<<grid, 256, 0, stream>>>(static_cast<const T*>(x), static_cast<const T*>(residual),
-                                                          static_cast<T*>(out), n, cut, scale, rng);
-    else
-        dropout_kernel<T, false><<<grid, 256, 0, stream>>>(static_cast<const T*>(x), nullptr, static_cast<T*>(out), n, cut,
-                                                           scale, rng);
+    // several groups per thread once there are enough to fill the GPU with such threads twice over
+    constexpr int kMany = sizeof(T) == 2 ? 4 : 2;
+    const bool many = groups >= 148ll * 2048 * kMany * 2;
+    const int64_t per_cta = 256 * (many ? kMany : 1), ctas = (groups + per_cta - 1) / per_cta;
+    if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+    const T* in = static_cast<const T*>(x);
+    const T* res = static_cast<const T*>(residual);
+    T* to = static_cast<T*>(out);
+    if (residual != nullptr) {
+        if (many) dropout_kernel<T, true, kMany><<<(unsigned)ctas, 256, 0, stream>>>(in, res, to, n, cut, scale, rng);
+        else dropout_kernel<T, true, 1><<<(unsigned)ctas, 256, 0, stream>>>(in, res, to, n, cut, scale, rng);
+    } else {
+        if (many) dropout_kernel<T, false, kMany><<<(unsigned)ctas, 256, 0, stream>>>(in, res, to, n, cut, scale, rng);
+        else dropout_kernel<T, false, 1><<<(unsigned)ctas, 256, 0, stream>>>(in, res, to, n, cut, scale, rng);
+    }
     return cudaGetLastError();
 }
 

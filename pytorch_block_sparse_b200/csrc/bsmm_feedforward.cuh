@@ -46,6 +46,28 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
         make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
+// the same as loaded, not yet widened: what a thread holds while loads are in flight
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = *reinterpret_cast<const float4*>(p);
+        b = *reinterpret_cast<const float4*>(p + 4);
+    }
+    __device__ __forceinline__ void unpack(float (&v)[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
+template <>
+struct Raw8<__nv_bfloat16> {
+    uint4 a;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void unpack(float (&v)[8]) const { unpack8(a, v); }
+};
+
 // The gate's activation, in fp32.  kind: 0 SiLU g / (1 + exp(-g)), 1 GELU (erf form).
 __device__ __forceinline__ float gate_act(float g, int kind) {
     if (kind == 0) return g / (1.f + expf(-g));
@@ -76,8 +98,8 @@ cudaError_t launch_gated_act_backward(const void* pre, const void* dh, int64_t m
                                       float* dbias, float* workspace, int act, bool pre_bf16, bool io_bf16,
                                       cudaStream_t stream);
 cudaError_t launch_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx,
-                               const float* data, int64_t hidden, const float* bias, void* h, int act, bool x_bf16,
-                               bool h_bf16, cudaStream_t stream);
+                               const float* data, int64_t nnz, int64_t hidden, const float* bias, void* h, int act,
+                               bool x_bf16, bool h_bf16, cudaStream_t stream);
 
 struct AdapterCall {
     const void* x;           // [tokens, inner]

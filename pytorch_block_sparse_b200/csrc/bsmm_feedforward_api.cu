@@ -69,7 +69,7 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
         return BSMM_ERR_INVALID_ARGUMENT;
     if (nnz > 0x7fffffff || too_large(m, k) || too_large(m, hidden) || (m + 7) / 8 > 65535) return BSMM_ERR_TOO_LARGE;
     const bool io16 = (flags & BSMM_GATED_IO_BF16) != 0;
-    return bsmm::report_cuda(bsmm::launch_gated_small(x, m, k, ptr, idx, data, hidden, bias, h, (flags & BSMM_GATED_GELU) != 0,
+    return bsmm::report_cuda(bsmm::launch_gated_small(x, m, k, ptr, idx, data, nnz, hidden, bias, h, (flags & BSMM_GATED_GELU) != 0,
                                                       io16 || (flags & BSMM_GATED_X_BF16) != 0, io16,
                                                       static_cast<cudaStream_t>(stream)));
 }

@@ -3,12 +3,15 @@
 // hidden units 32 j ... 32 j + 31, the next 32 their u.  (Wg and Wu are one block-sparse matrix of 2 hidden rows whose
 // block-rows alternate the same way, so one product computes `pre`, and the gradients with respect to the input and to
 // both weights are one product each.)
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include "bsmm_feedforward.cuh"
 
 namespace bsmm {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kRowsPerChunk = 256;  // rows whose bias gradient one CTA adds up
 
@@ -104,70 +107,277 @@ sum_chunks_kernel(const float* __restrict__ partial, int64_t chunks, int64_t col
 }
 
 // Few tokens: h straight from the stored fp32 blocks, exact fp32 products, no weight images.  Bound by reading the
-// blocks (4 KiB each) once.  A CTA takes one block-row of hidden units: warps 0-3 walk the gate's blocks, 4-7 the up
-// projection's.  data[slot][c][r]: lane (q, r4) of a warp holds the four outputs r = 4 r4 ... of the inputs c = 8 q ... 8 q + 7
-// of a block, so that it loads eight 16-byte pieces of weights (each warp load covers four 128-byte rows) and eight
-// consecutive inputs of a token; the four q and four warps are added up at the end, in a fixed order.
-constexpr int kSmallTokens = 8;
+// blocks (4 KiB each) once.  A cluster of `parts` CTAs takes one block-row of hidden units; in each CTA warps 0-3 walk the
+// gate's blocks, 4-7 the up projection's, a block per warp and step.  data[slot][c][r]: lane (q, r4) of a warp holds the
+// four outputs r = 4 r4 ... of the inputs c = 8 q ... 8 q + 7.  Every warp has a ring of its own in shared memory, filled by
+// cp.async (16 bytes per lane, a lane reads back the weights it copied itself) kStages - 1 blocks ahead, because a warp that
+// waits for its block before it asks for the next keeps only 4 KiB in flight.  The four q, the warps and the CTAs of the
+// cluster (through distributed shared memory) are added up at the end in a fixed order.
+constexpr int kSmallStages = 3;
 
-template <typename X, typename H>
-__global__ void __launch_bounds__(256, 2)
-gated_small_kernel(const X* __restrict__ x, int64_t m, int64_t k, const int32_t* __restrict__ ptr,
-                   const int2* __restrict__ idx, const float* __restrict__ data, int64_t hidden,
-                   const float* __restrict__ bias, H* __restrict__ h, int act) {
-    __shared__ float sums[8][kSmallTokens][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane >> 3, r4 = lane & 7;
-    const int64_t block = blockIdx.x, t0 = (int64_t)blockIdx.y * kSmallTokens;
-    const int nt = (int)min((int64_t)kSmallTokens, m - t0);
-    const int64_t row = 2 * block + (warp >> 2);
-    float acc[kSmallTokens][4];
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// w = parts[0] + parts[1] + parts[2] exactly (3 x 8 significant bits), for a pair of values
+__device__ __forceinline__ void split3_bf16x2(float w0, float w1, uint32_t (&parts)[3]) {
+    asm("{\n\t.reg .b16 h0, h1, m1;\n\t.reg .f32 d0, d1;\n\t"
+        "mov.b16 m1, 0xBF80;\n\t"
+        "cvt.rn.bf16x2.f32 %0, %4, %3;\n\t"
+        "mov.b32 {h0, h1}, %0;\n\t"
+        "fma.rn.f32.bf16 d0, h0, m1, %3;\n\t"
+        "fma.rn.f32.bf16 d1, h1, m1, %4;\n\t"
+        "cvt.rn.bf16x2.f32 %1, d1, d0;\n\t"
+        "mov.b32 {h0, h1}, %1;\n\t"
+        "fma.rn.f32.bf16 d0, h0, m1, d0;\n\t"
+        "fma.rn.f32.bf16 d1, h1, m1, d1;\n\t"
+        "cvt.rn.bf16x2.f32 %2, d1, d0;\n\t}"
+        : "=&r"(parts[0]), "=&r"(parts[1]), "=r"(parts[2])
+        : "f"(w0), "f"(w1));
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename X, int kTok>
+struct SmallSmem {
+    static constexpr int kXBytes = kTok * 32 * (int)sizeof(X);  // a block's inputs, [token][32]
+    static constexpr int kStage = 4096 + kXBytes;
+    static constexpr int kRing = kSmallStages * kStage;         // per warp
+    static constexpr int kTotal = 8 * kRing;                    // at the end [8 warps][kTok][32] fp32 and [2][kTok][32]
+    static_assert(kTotal >= (8 + 2) * kTok * 128, "the sums reuse the rings");
+};
+
+// How a warp multiplies a block with its tokens' inputs, and where its sums lie.  Weights in the ring: row c at c * 128, its
+// 16-byte piece r4 at position r4 ^ (2 (c / 8)), so that the four c / 8 of a quarter-warp's loads never share a bank.
+//
+// CUDA cores, exact fp32: acc[t][j] of lane (q, r4) belongs to output 4 r4 + j and this lane's inputs 8 q ... 8 q + 7.
+template <typename X, int kTok>
+struct SmallFma {
+    float acc[kTok][4];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int t = 0; t < kSmallTokens; ++t)
+        for (int t = 0; t < kTok; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+    }
+    __device__ __forceinline__ void block(const float4 (&w)[8], const X* xs, int nt, int lane) {
+        const X* mine = xs + (lane & 3) * 8;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[t][j] = 0.f;
-    const int end = ptr[row + 1];
-    for (int e = ptr[row] + (warp & 3); e < end; e += 4) {
-        const int2 entry = __ldg(idx + e);
-        const float4* w4 = reinterpret_cast<const float4*>(data + (int64_t)entry.y * kBlockElems + q * 256) + r4;
-        float4 w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = __ldg(w4 + i * 8);
-        const X* xe = x + t0 * k + (int64_t)entry.x * 32 + q * 8;
-#pragma unroll
-        for (int t = 0; t < kSmallTokens; ++t) {
+        for (int t = 0; t < kTok; ++t) {
             if (t < nt) {
                 float xv[8];
-                load8(xe + t * k, xv);
+                load8(mine + t * 32, xv);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    acc[t][0] = fmaf(w[i].x, xv[i], acc[t][0]);
-                    acc[t][1] = fmaf(w[i].y, xv[i], acc[t][1]);
-                    acc[t][2] = fmaf(w[i].z, xv[i], acc[t][2]);
-                    acc[t][3] = fmaf(w[i].w, xv[i], acc[t][3]);
+                for (int j = 0; j < 8; ++j) {
+                    acc[t][0] = fmaf(w[j].x, xv[j], acc[t][0]);
+                    acc[t][1] = fmaf(w[j].y, xv[j], acc[t][1]);
+                    acc[t][2] = fmaf(w[j].z, xv[j], acc[t][2]);
+                    acc[t][3] = fmaf(w[j].w, xv[j], acc[t][3]);
                 }
             }
         }
     }
+    __device__ __forceinline__ void store(float* sums, int lane) {  // [kTok][32]
 #pragma unroll
-    for (int t = 0; t < kSmallTokens; ++t) {
+        for (int t = 0; t < kTok; ++t) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            acc[t][j] += __shfl_xor_sync(0xffffffffu, acc[t][j], 8);
-            acc[t][j] += __shfl_xor_sync(0xffffffffu, acc[t][j], 16);
+            for (int j = 0; j < 4; ++j) {
+                acc[t][j] += __shfl_xor_sync(0xffffffffu, acc[t][j], 1);
+                acc[t][j] += __shfl_xor_sync(0xffffffffu, acc[t][j], 2);
+            }
+            if ((lane & 3) == 0)
+                *reinterpret_cast<float4*>(sums + t * 32 + (lane >> 2) * 4) = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
         }
-        if (q == 0) *reinterpret_cast<float4*>(&sums[warp][t][r4 * 4]) = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
     }
+};
+// Tensor cores, bf16 inputs: the block transposed is the 32 x 32 left operand of mma.m16n8k16, eight tokens the right one.
+// A weight is the sum of three bf16 values exactly, so that every product is exact and only the fp32 sums round, as with
+// fused multiply-adds.  Rows of a fragment are outputs 4 r4 + 2 i, + 1 and its contraction indices this lane's
+// inputs 8 q + 4 s ... + 3 (both operands permuted alike): the lane already holds them.
+template <int kTok>
+struct SmallMma {
+    float acc[kTok / 8][2][4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < kTok / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
+    }
+    __device__ __forceinline__ void block(const float4 (&w)[8], const __nv_bfloat16* xs, int nt, int lane) {
+        uint4 b[kTok / 8];
+#pragma unroll
+        for (int n = 0; n < kTok / 8; ++n) b[n] = *reinterpret_cast<const uint4*>(xs + (n * 8 + (lane >> 2)) * 32 + (lane & 3) * 8);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            uint32_t low[4][3], high[4][3];  // output 4 r4 + e: pairs of inputs 4 s, 4 s + 1 and 4 s + 2, 4 s + 3
+            split3_bf16x2(w[4 * s].x, w[4 * s + 1].x, low[0]);
+            split3_bf16x2(w[4 * s].y, w[4 * s + 1].y, low[1]);
+            split3_bf16x2(w[4 * s].z, w[4 * s + 1].z, low[2]);
+            split3_bf16x2(w[4 * s].w, w[4 * s + 1].w, low[3]);
+            split3_bf16x2(w[4 * s + 2].x, w[4 * s + 3].x, high[0]);
+            split3_bf16x2(w[4 * s + 2].y, w[4 * s + 3].y, high[1]);
+            split3_bf16x2(w[4 * s + 2].z, w[4 * s + 3].z, high[2]);
+            split3_bf16x2(w[4 * s + 2].w, w[4 * s + 3].w, high[3]);
+#pragma unroll
+            for (int n = 0; n < kTok / 8; ++n) {
+                const uint32_t b0 = s == 0 ? b[n].x : b[n].z, b1 = s == 0 ? b[n].y : b[n].w;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int part = 0; part < 3; ++part)
+                        mma16816(acc[n][i], low[2 * i][part], low[2 * i + 1][part], high[2 * i][part], high[2 * i + 1][part], b0, b1);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float* sums, int lane) {
+        const int r = (lane >> 2) * 4, t = (lane & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < kTok / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float* to = sums + (n * 8 + t) * 32 + r + 2 * i;
+                *reinterpret_cast<float2*>(to) = make_float2(acc[n][i][0], acc[n][i][2]);
+                *reinterpret_cast<float2*>(to + 32) = make_float2(acc[n][i][1], acc[n][i][3]);
+            }
+    }
+};
+
+template <typename X, typename H, int kTok, typename Math>
+__global__ void __launch_bounds__(256)
+gated_small_kernel(const X* __restrict__ x, int64_t m, int64_t k, const int32_t* __restrict__ ptr,
+                   const int2* __restrict__ idx, const float* __restrict__ data, int64_t hidden,
+                   const float* __restrict__ bias, H* __restrict__ h, int act, int parts) {
+    using S = SmallSmem<X, kTok>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, r4 = lane >> 2;
+    const int64_t block = blockIdx.x / parts, t0 = (int64_t)blockIdx.y * kTok;
+    const int part = (int)(blockIdx.x % parts);
+    const int nt = (int)min((int64_t)kTok, m - t0);
+    const int64_t row = 2 * block + (warp >> 2);
+    const int begin = ptr[row] + part * 4 + (warp & 3), stride = 4 * parts;
+    const int count = max(0, (ptr[row + 1] - begin + stride - 1) / stride);
+    uint8_t* ring = smem + warp * S::kRing;
+    const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
+    const int place = ((r4 ^ (2 * q)) << 4) + q * 1024;  // of this lane's first piece in a stage
+
+    int2 ents = make_int2(0, 0);  // entry i of this warp is held by lane i mod 32
+    auto issue = [&](int i) {
+        if (i < count) {
+            if ((i & 31) == 0) ents = i + lane < count ? __ldg(idx + begin + (i + lane) * stride) : make_int2(0, 0);
+            const int col = __shfl_sync(0xffffffffu, ents.x, i & 31), slot = __shfl_sync(0xffffffffu, ents.y, i & 31);
+            const uint32_t stage = ring_addr + (i % kSmallStages) * S::kStage;
+            const float* w = data + (int64_t)slot * kBlockElems + q * 256 + r4 * 4;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) copy16(stage + place + j * 128, w + j * 32);
+            constexpr int kPieces = S::kXBytes / kTok / 16;  // of a token
+#pragma unroll
+            for (int piece = lane; piece < kTok * kPieces; piece += 32) {
+                const int t = piece / kPieces, o = piece % kPieces;
+                if (t < nt)
+                    copy16(stage + 4096 + piece * 16, reinterpret_cast<const uint8_t*>(x + (t0 + t) * k + (int64_t)col * 32) + o * 16);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    Math math;
+    math.clear();
+#pragma unroll
+    for (int i = 0; i < kSmallStages - 1; ++i) issue(i);
+    for (int i = 0; i < count; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kSmallStages - 2) : "memory");
+        __syncwarp();  // every lane's part of the block's inputs has arrived, and the stage of the next copy has been read
+        issue(i + kSmallStages - 1);
+        const uint8_t* stage = ring + (i % kSmallStages) * S::kStage;
+        float4 w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const float4*>(stage + place + j * 128);
+        math.block(w, reinterpret_cast<const X*>(stage + 4096), nt, lane);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the rings have been read: their memory takes the sums
+    float* sums = reinterpret_cast<float*>(smem);
+    math.store(sums + warp * kTok * 32, lane);
     __syncthreads();
-    const int t = threadIdx.x >> 5;  // one output per thread
-    if (t < nt) {
-        float g = sums[0][t][lane] + sums[1][t][lane] + sums[2][t][lane] + sums[3][t][lane];
-        float u = sums[4][t][lane] + sums[5][t][lane] + sums[6][t][lane] + sums[7][t][lane];
-        if (bias != nullptr) {
-            g += bias[block * 64 + lane];
-            u += bias[block * 64 + 32 + lane];
-        }
-        h[(t0 + t) * hidden + block * 32 + lane] = from_float<H>(gate_act(g, act) * u);
+    float* both = sums + 8 * kTok * 32;  // this CTA's sums: [gate, up][kTok][32]
+    for (int i = threadIdx.x; i < 2 * kTok * 32; i += 256) {
+        const float* s = sums + (i / (kTok * 32)) * 4 * kTok * 32 + i % (kTok * 32);
+        both[i] = s[0] + s[kTok * 32] + s[2 * kTok * 32] + s[3 * kTok * 32];
     }
+    cg::cluster_group cluster = cg::this_cluster();
+    if (parts > 1) cluster.sync(); else __syncthreads();
+    // the cluster's CTAs share the outputs among them
+    for (int i = part * 256 + threadIdx.x; i < nt * 32; i += parts * 256) {
+        float g = 0.f, u = 0.f;
+        for (int c = 0; c < parts; ++c) {
+            const float* theirs = parts > 1 ? cluster.map_shared_rank(both, c) : both;
+            g += theirs[i];
+            u += theirs[kTok * 32 + i];
+        }
+        const int t = i >> 5, r = i & 31;
+        if (bias != nullptr) {
+            g += bias[block * 64 + r];
+            u += bias[block * 64 + 32 + r];
+        }
+        h[(t0 + t) * hidden + block * 32 + r] = from_float<H>(gate_act(g, act) * u);
+    }
+    if (parts > 1) cluster.sync();  // nobody leaves while its sums are read
+}
+
+template <typename X, typename H, int kTok, typename Math>
+cudaError_t small(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, const float* data, int64_t nnz,
+                  int64_t hidden, const float* bias, void* h, int act, cudaStream_t stream) {
+    constexpr int kBytes = SmallSmem<X, kTok>::kTotal;
+    constexpr int kMaxDevices = 64;
+    static bool ready[kMaxDevices] = {false};  // the attribute is per device; threads racing on the first call set it twice
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    if (!ready[dev]) {
+        err = cudaFuncSetAttribute(gated_small_kernel<X, H, kTok, Math>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        if (err != cudaSuccess) return err;
+        ready[dev] = true;
+    }
+    const int64_t rows = hidden / 32, tiles = (m + kTok - 1) / kTok;
+    if (tiles > 65535) return cudaErrorInvalidValue;
+    // as many CTAs per block-row as fill the GPU twice over, while every warp has a block of its own
+    int parts = 1;
+    while (parts < 8 && rows * tiles * parts * 2 <= 2 * 148 && nnz / rows >= parts * 2 * 8) parts *= 2;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(rows * parts), (unsigned)tiles);
+    config.blockDim = dim3(256);
+    config.dynamicSmemBytes = kBytes;
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, gated_small_kernel<X, H, kTok, Math>, static_cast<const X*>(x), m, k, ptr,
+                              reinterpret_cast<const int2*>(idx), data, hidden, bias, static_cast<H*>(h), act, parts);
+}
+
+template <typename H>
+cudaError_t small_fp32(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, const float* data,
+                       int64_t nnz, int64_t hidden, const float* bias, void* h, int act, cudaStream_t stream) {
+    if (m == 1) return small<float, H, 1, SmallFma<float, 1>>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream);
+    if (m <= 4) return small<float, H, 4, SmallFma<float, 4>>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream);
+    return small<float, H, 8, SmallFma<float, 8>>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream);
+}
+
+template <typename H>
+cudaError_t small_bf16(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, const float* data,
+                       int64_t nnz, int64_t hidden, const float* bias, void* h, int act, cudaStream_t stream) {
+    using X = __nv_bfloat16;
+    if (m == 1) return small<X, H, 1, SmallFma<X, 1>>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream);
+    if (m <= 8) return small<X, H, 8, SmallMma<8>>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream);
+    if (m <= 16) return small<X, H, 16, SmallMma<16>>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream);
+    return small<X, H, 32, SmallMma<32>>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream);
 }
 
 template <typename P, typename H>
@@ -222,26 +432,13 @@ cudaError_t launch_gated_act_backward(const void* pre, const void* dh, int64_t m
 }
 
 cudaError_t launch_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx,
-                               const float* data, int64_t hidden, const float* bias, void* h, int act, bool x_bf16,
-                               bool h_bf16, cudaStream_t stream) {
+                               const float* data, int64_t nnz, int64_t hidden, const float* bias, void* h, int act,
+                               bool x_bf16, bool h_bf16, cudaStream_t stream) {
     if (m == 0 || hidden == 0) return cudaSuccess;
-    const int64_t tiles = (m + kSmallTokens - 1) / kSmallTokens;
-    if (tiles > 65535 || hidden / 32 > 0x7fffffffll) return cudaErrorInvalidValue;
-    const dim3 grid((unsigned)(hidden / 32), (unsigned)tiles);
-    const int2* idx2 = reinterpret_cast<const int2*>(idx);
-    if (x_bf16) {
-        const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);
-        if (h_bf16)
-            gated_small_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, stream>>>(
-                xb, m, k, ptr, idx2, data, hidden, bias, static_cast<__nv_bfloat16*>(h), act);
-        else
-            gated_small_kernel<__nv_bfloat16, float><<<grid, 256, 0, stream>>>(xb, m, k, ptr, idx2, data, hidden, bias,
-                                                                               static_cast<float*>(h), act);
-    } else {
-        gated_small_kernel<float, float><<<grid, 256, 0, stream>>>(static_cast<const float*>(x), m, k, ptr, idx2, data, hidden,
-                                                                   bias, static_cast<float*>(h), act);
-    }
-    return cudaGetLastError();
+    if (hidden / 32 * 8 > 0x7fffffffll) return cudaErrorInvalidValue;
+    if (!x_bf16) return small_fp32<float>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream);
+    return h_bf16 ? small_bf16<__nv_bfloat16>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream)
+                  : small_bf16<float>(x, m, k, ptr, idx, data, nnz, hidden, bias, h, act, stream);
 }
 
 }  // namespace bsmm

@@ -147,30 +147,31 @@ class BlockSparseGatedLinear(nn.Module):
         return split_rows(self.weight.to_dense())
 
     def forward(self, x):
-        if x.dim() < 2:
-            raise Exception(f"Invalid dimensions for x {tuple(x.shape)} : x should have at least 2 dimensions.")
-        if x.shape[-1] != self.in_features:
+        weight, bias = self.weight, self.bias
+        data = weight.get_differentiable_data()
+        shape = x.shape
+        if len(shape) < 2:
+            raise Exception(f"Invalid dimensions for x {tuple(shape)} : x should have at least 2 dimensions.")
+        if shape[-1] != self.in_features:
             raise Exception("Invalid matrices sizes (%d, %d) x (%d, %d)" % (
-                x.numel() // max(1, x.shape[-1]), x.shape[-1], self.in_features, 2 * self.hidden_features))
-        if x.dtype not in (torch.float32, torch.bfloat16):
+                x.numel() // max(1, shape[-1]), shape[-1], self.in_features, 2 * self.hidden_features))
+        if x.dtype is not torch.float32 and x.dtype is not torch.bfloat16:
             raise ValueError("BlockSparseGatedLinear takes float32 or bfloat16 tensors, got %s" % x.dtype)
-        self.weight._require_cuda()
-        if x.device != self.weight.data.device:
-            raise native.NativeError("x is on %s, the layer on %s" % (x.device, self.weight.data.device))
-        lead = x.shape[:-1]
-        flat = x.reshape(-1, self.in_features).contiguous()
-        data = self.weight.get_differentiable_data()
-        if torch.is_grad_enabled() and (x.requires_grad or data.requires_grad or (self.bias is not None and self.bias.requires_grad)):
-            h = BlockSparseGatedFunction.apply(flat, data, self.weight, self.bias, self.activation, self.precision)
+        if not data.is_cuda:
+            weight._require_cuda()
+        if x.device != data.device:
+            raise native.NativeError("x is on %s, the layer on %s" % (x.device, data.device))
+        flat = (x if len(shape) == 2 else x.reshape(-1, shape[-1])).contiguous()
+        if torch.is_grad_enabled() and (x.requires_grad or data.requires_grad or (bias is not None and bias.requires_grad)):
+            h = BlockSparseGatedFunction.apply(flat, data, weight, bias, self.activation, self.precision)
         else:
-            h = self._infer(flat)
-        return h.reshape(*lead, self.hidden_features)
+            h = self._infer(flat, weight, bias, data)
+        return h if len(shape) == 2 else h.reshape(*shape[:-1], self.hidden_features)
 
-    def _infer(self, flat):
-        weight, bias = self.weight, self.bias.detach() if self.bias is not None else None
+    def _infer(self, flat, weight, bias, data):
         out_dtype = _out_dtype(flat, self.precision)
         if flat.shape[0] <= SMALL_TOKENS:
-            return native.gated_small(flat, weight.row_start_ends_a, weight.cols_a, weight.data, self.hidden_features, bias,
+            return native.gated_small(flat, weight.row_start_ends_a, weight.cols_a, data, self.hidden_features, bias,
                                       self.activation, out_dtype)
         pre = weight.reverse_matmul(flat.float(), transpose=True, bias=bias, precision=self.precision)
         return native.gated_act(pre, self.activation, out_dtype)

@@ -196,7 +196,7 @@ def resolve_precision(precision):
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()  # (an int: ctypes converts it faster than it builds a c_void_p)
 
 
 def _aligned(t, alignment=16):
@@ -210,7 +210,25 @@ def _aligned(t, alignment=16):
 
 
 def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _Here:
+    """The guard of a call whose device is the current one already: nothing to set, nothing to put back."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """``torch.cuda.device(device)``, which costs a few microseconds, only where another device is current."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _need_cuda(t, name):
@@ -237,7 +255,7 @@ def pack_weights(data, precision):
     sumsq = torch.empty(nnz, dtype=torch.float32, device=data.device)
     nbytes = lib.bsmm_packed_bytes(nnz, precision)
     images = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=data.device) if nbytes > 0 else None
-    with torch.cuda.device(data.device):
+    with _on(data.device):
         check(
             lib.bsmm_pack_weights(_ptr(raw), nnz, precision, _ptr(images), _ptr(sumsq), _stream(data.device)),
             "bsmm_pack_weights",
@@ -256,7 +274,7 @@ def block_sumsq(data):
         raw = raw.contiguous()
     raw = _aligned(raw)
     sumsq = torch.empty(nnz, dtype=torch.float32, device=data.device)
-    with torch.cuda.device(data.device):
+    with _on(data.device):
         check(lib.bsmm_pack_weights(_ptr(raw), nnz, PREC_FP32_SIMT, None, _ptr(sumsq), _stream(data.device)),
               "bsmm_pack_weights")
     return sumsq
@@ -266,7 +284,7 @@ def rebuild_indices(blocks, n_block_rows, n_block_cols, cell_slot, row_ptr, cols
     """``bsmm_rebuild_indices``: CSR / CSC buffers (written in place) from the slot-order ``blocks`` list."""
     _need_cuda(blocks, "blocks")
     lib = load()
-    with torch.cuda.device(blocks.device):
+    with _on(blocks.device):
         check(
             lib.bsmm_rebuild_indices(
                 _ptr(blocks), blocks.shape[0] // 2, n_block_rows, n_block_cols, _ptr(cell_slot), _ptr(row_ptr),
@@ -282,7 +300,7 @@ def select_lowest(stat, k):
     lib = load()
     stat = stat.detach().contiguous()
     out = torch.empty(k, dtype=torch.int32, device=stat.device)
-    with torch.cuda.device(stat.device):
+    with _on(stat.device):
         check(lib.bsmm_select_lowest(_ptr(stat), stat.shape[0], k, _ptr(out), _stream(stat.device)), "bsmm_select_lowest")
     return out
 
@@ -293,7 +311,7 @@ def sample_free_cells(cell_slot, n_free, k, seed, status):
     lib = load()
     scratch = torch.empty(max(n_free, 1), dtype=torch.int32, device=cell_slot.device)
     out = torch.empty(k, dtype=torch.int32, device=cell_slot.device)
-    with torch.cuda.device(cell_slot.device):
+    with _on(cell_slot.device):
         check(
             lib.bsmm_sample_free_cells(
                 _ptr(cell_slot), cell_slot.numel(), n_free, k, ctypes.c_uint64(seed & 0xFFFFFFFFFFFFFFFF), _ptr(scratch),
@@ -307,7 +325,7 @@ def sample_free_cells(cell_slot, n_free, k, seed, status):
 def move_blocks(blocks, slots, cells, n_block_cols, status):
     """``bsmm_move_blocks``: ``blocks[slots[j]]`` becomes position ``cells[j]`` (in place)."""
     lib = load()
-    with torch.cuda.device(blocks.device):
+    with _on(blocks.device):
         check(
             lib.bsmm_move_blocks(
                 _ptr(blocks), _ptr(slots), _ptr(cells), slots.shape[0], n_block_cols, blocks.shape[0] // 2, _ptr(status),
@@ -344,7 +362,7 @@ class DsdPlan:
             if nbytes < 0:
                 raise NativeError("invalid plan group %r" % (group,))
             buf = torch.empty(nbytes, dtype=torch.uint8, device=self.ptr.device)
-            with torch.cuda.device(self.ptr.device):
+            with _on(self.ptr.device):
                 check(
                     lib.bsmm_build_plan(
                         _ptr(self.ptr), _ptr(self.idx), self.n_out_blocks, self.nnz, group, _ptr(buf),
@@ -407,7 +425,7 @@ def dsd_matmul(a, plan, packed, n_out, transpose, bias=None, out=None, out_colma
     if pre_activation is not None and (pre_activation.dtype != torch.float32 or not pre_activation.is_contiguous()
                                        or pre_activation.numel() != m * n_out):
         raise NativeError("pre_activation must be a contiguous float32 tensor of the output's size")
-    with torch.cuda.device(a.device):
+    with _on(a.device):
         check(
             lib.bsmm_dsd_multi(
                 _ptr(a), m, k, _ptr(plan.ptr), _ptr(plan.idx), plan.nnz, _ptr(packed.data), _ptr(packed.images),
@@ -438,7 +456,7 @@ def dsd_scatter(a, plan, packed, n_out, transpose, parts, slot, scratch=None):
     group = plan.group_for(m, prec)
     flags = prec | (0 if transpose else DSD_DGRAD) | (group << 8)
     part_array = (ctypes.c_void_p * len(parts))(*[ctypes.c_void_p(int(ptr)) for ptr in parts])
-    with torch.cuda.device(a.device):
+    with _on(a.device):
         check(
             lib.bsmm_dsd_scatter(
                 _ptr(a), m, k, _ptr(plan.ptr), _ptr(plan.idx), plan.nnz, _ptr(packed.data), _ptr(packed.images),
@@ -457,7 +475,7 @@ def sum_row_slots(parts, outs, out_row0):
     lib = load()
     slots, rows, cols = parts.shape
     out_array = (ctypes.c_void_p * len(outs))(*[ctypes.c_void_p(int(ptr)) for ptr in outs])
-    with torch.cuda.device(parts.device):
+    with _on(parts.device):
         check(
             lib.bsmm_sum_row_slots(_ptr(parts), slots, rows, cols, out_array, len(outs), out_row0, _stream(parts.device)),
             "bsmm_sum_row_slots",
@@ -470,7 +488,7 @@ def allreduce_peers(bufs, rank, elems, scale, device):
     lib = load()
     arr = (ctypes.c_void_p * len(bufs))(*[ctypes.c_void_p(int(ptr)) for ptr in bufs])
     with torch.cuda.device(device):
-        check(lib.bsmm_allreduce_peers(arr, len(bufs), rank, elems, ctypes.c_float(scale), _stream(device)),
+        check(lib.bsmm_allreduce_peers(arr, len(bufs), rank, elems, ctypes.c_float(scale), torch.cuda.current_stream(device).cuda_stream),
               "bsmm_allreduce_peers")
 
 
@@ -485,7 +503,7 @@ class SddmmPlan:
         n_rows = ptr.shape[0] - 1
         nnz = idx.shape[0]
         self.buffer = torch.empty(lib.bsmm_sddmm_plan_bytes(n_rows, nnz), dtype=torch.uint8, device=ptr.device)
-        with torch.cuda.device(ptr.device):
+        with _on(ptr.device):
             check(
                 lib.bsmm_build_sddmm_plan(_ptr(ptr), n_rows, nnz, _ptr(self.buffer), _stream(ptr.device)),
                 "bsmm_build_sddmm_plan",
@@ -520,7 +538,7 @@ def sddmm_static(a, b, blocks, out, plan, block_sumsq=None, precision=None):
     tokens, rows = a.shape
     cols = b.shape[1]
     nnz = blocks.shape[0] // 2
-    with torch.cuda.device(a.device):
+    with _on(a.device):
         check(
             lib.bsmm_sddmm_static(
                 _ptr(a), _ptr(b), rows, cols, tokens, _ptr(out), _ptr(blocks), nnz, _ptr(plan.idx), _ptr(plan.buffer),
@@ -551,7 +569,7 @@ def sddmm(a, a_rowmajor, b, b_rowmajor, blocks, out, precision=None, block_sumsq
     flags |= SDDMM_IO_BF16 if io16 else 0
     ws_bytes = lib.bsmm_sddmm_workspace_bytes(rows, cols, tokens, nnz, flags) if plan is not None else 0
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=a.device) if ws_bytes > 0 else None
-    with torch.cuda.device(a.device):
+    with _on(a.device):
         check(
             lib.bsmm_sddmm(
                 _ptr(a), _ptr(b), rows, cols, tokens, _ptr(out), _ptr(blocks), nnz,
@@ -577,7 +595,7 @@ def gated_act(pre, activation, out_dtype):
     out = torch.empty((m, hidden), dtype=out_dtype, device=pre.device)
     flags = _gated_flags(activation) | (GATED_IO_BF16 if out_dtype == torch.bfloat16 else 0)
     flags |= GATED_PRE_BF16 if pre.dtype == torch.bfloat16 else 0
-    with torch.cuda.device(pre.device):
+    with _on(pre.device):
         check(load().bsmm_gated_act(_ptr(pre), m, hidden, _ptr(out), flags, _stream(pre.device)), "bsmm_gated_act")
     return out
 
@@ -595,7 +613,7 @@ def gated_act_backward(pre, dh, activation, want_bias):
         ws = torch.empty(max(16, lib.bsmm_gated_act_workspace_bytes(m, hidden)), dtype=torch.uint8, device=pre.device)
     flags = _gated_flags(activation) | (GATED_IO_BF16 if dh.dtype == torch.bfloat16 else 0)
     flags |= GATED_PRE_BF16 if pre.dtype == torch.bfloat16 else 0
-    with torch.cuda.device(pre.device):
+    with _on(pre.device):
         check(
             lib.bsmm_gated_act_backward(_ptr(pre), _ptr(_aligned(dh)), m, hidden, _ptr(dpre), _ptr(dbias), _ptr(ws), flags,
                                         _stream(pre.device)),
@@ -613,8 +631,8 @@ def gated_small(x, ptr, idx, data, hidden, bias, activation, out_dtype):
     flags = _gated_flags(activation)
     if x.dtype == torch.bfloat16:
         flags |= GATED_IO_BF16 if out_dtype == torch.bfloat16 else GATED_X_BF16
-    x, ptr, idx, data, bias = _aligned(x), _aligned(ptr), _aligned(idx), _aligned(data.detach()), _aligned(bias)
-    with torch.cuda.device(x.device):
+    x, ptr, idx, data, bias = _aligned(x), _aligned(ptr, 4), _aligned(idx, 8), _aligned(data), _aligned(bias, 4)
+    with _on(x.device):
         check(
             load().bsmm_gated_small(_ptr(x), m, k, _ptr(ptr), _ptr(idx), idx.shape[0], _ptr(data), hidden, _ptr(bias),
                                     _ptr(out), flags, _stream(x.device)),
@@ -631,7 +649,7 @@ def dropout(x, residual, cut, rng):
     residual = _aligned(residual)
     out = torch.empty_like(x)
     flags = DROPOUT_BF16 if x.dtype == torch.bfloat16 else 0
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         check(load().bsmm_dropout(_ptr(x), _ptr(residual), _ptr(out), x.numel(), cut, _ptr(rng), flags, _stream(x.device)),
               "bsmm_dropout")
     return out
@@ -641,7 +659,7 @@ def rng_next(state):
     """The (seed, counter) to draw with now, as a new int64 ``[2]`` tensor; the state's counter moves on (``bsmm_rng_next``)."""
     _need_cuda(state, "state")
     used = torch.empty(2, dtype=torch.int64, device=state.device)
-    with torch.cuda.device(state.device):
+    with _on(state.device):
         check(load().bsmm_rng_next(_ptr(state), _ptr(used), _stream(state.device)), "bsmm_rng_next")
     return used
 
@@ -656,7 +674,7 @@ def adapters(x, offsets, ids, down, up, scaling, base, out):
     x = _aligned(x)
     ws = torch.empty(max(16, lib.bsmm_adapters_workspace_bytes(tokens, inner, rank)), dtype=torch.uint8, device=x.device)
     flags = (ADAPTERS_IN_BF16 if x.dtype == torch.bfloat16 else 0) | (ADAPTERS_OUT_BF16 if out.dtype == torch.bfloat16 else 0)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         check(
             lib.bsmm_adapters(_ptr(x), tokens, inner, up.shape[1], _ptr(offsets), _ptr(ids), ids.shape[0], count, rank,
                               _ptr(down), _ptr(up), _ptr(scaling), _ptr(base), _ptr(out), _ptr(ws), flags, _stream(x.device)),
