@@ -3,14 +3,20 @@
 //
 // Two launches: the shrink kernel writes v[t] = x[t] D_a^T in fp32 (partial sums over ranges of the input features when
 // few tokens would leave SMs idle), the expand kernel adds the partial sums in order, scales and multiplies by U_a.
-// Both are memory bound (2 rank FLOP per input byte): one warp owns 16 tokens and works with mma.m16n8k16 on fragments
-// loaded straight from global memory, 16 bytes per lane.  The contraction index of such a product may be permuted as long
-// as both operands agree, so a lane takes eight CONSECUTIVE k of its row -- the four pairs that two instructions want
-// from it -- and nothing passes through shared memory; the output columns of four instructions are permuted the same
-// way so that a lane ends with eight consecutive columns of each of its two rows.
-// A warp walks the distinct adapters among its tokens.  With many short requests the walk is shared between `subs` warps.
-// fp32 tensors: both operands are split into bf16 hi + lo parts and three products are added (about 2^-16 relative per
-// term); bf16 tensors: x D is one product, v is split (its rounding to bf16 would cost as much as the output's own).
+// Both are memory bound and work with mma.sync on fragments of 16 bytes per lane.  The contraction index of such a product
+// may be permuted as long as both operands agree, so a lane takes eight CONSECUTIVE k of its row -- what two (bf16) or four
+// (tf32) instructions want from it -- and the output columns of four instructions are permuted the same way, so that a
+// lane ends with eight consecutive columns of each of its two rows.
+//
+// Two forms of each kernel, chosen by the average number of tokens per request:
+//   warps   (few tokens per request) a warp owns 16 tokens and walks the distinct adapters among them on its own, fragments
+//           straight from global memory; with many short requests the walk is shared between `subs` warps
+//   tiles   (prompts) a CTA owns 128 tokens and walks their adapters; the adapter's matrix passes through shared memory
+//           once for its eight warps, where the first form reads it once per 16 tokens
+//
+// Arithmetic.  fp32 tensors: both operands are split into tf32 hi + lo parts and three products are added (about 2^-21
+// relative per term); bf16 tensors: x D is one exact product, v is split into bf16 hi + lo (its rounding to one bf16 would
+// cost as much as the output's own).
 #include <cuda_bf16.h>
 
 #include "bsmm_feedforward.cuh"
@@ -26,49 +32,128 @@ constexpr int kNone = -1;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// kPairs pairs of consecutive values as bf16 pairs: hi parts, and lo parts (what hi leaves) of fp32 values
-template <typename T, int kPairs>
+__device__ __forceinline__ void mma1688(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// kLen (4 or 8) consecutive values of a row as an operand: bf16 pairs, or tf32 hi and lo parts
+template <typename T, int kLen>
 struct Fragment;
-template <int kPairs>
-struct Fragment<__nv_bfloat16, kPairs> {
-    static constexpr bool kSplit = false;
-    uint32_t hi[kPairs];
+template <int kLen>
+struct Fragment<__nv_bfloat16, kLen> {
+    uint32_t hi[kLen / 2];
     __device__ __forceinline__ void load(const __nv_bfloat16* p) {
-        if (kPairs == 4) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-            hi[0] = w.x; hi[1] = w.y; hi[2 % kPairs] = w.z; hi[3 % kPairs] = w.w;
+        if constexpr (kLen == 8) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p);
+            hi[0] = w.x; hi[1] = w.y; hi[2] = w.z; hi[3] = w.w;
         } else {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+            const uint2 w = *reinterpret_cast<const uint2*>(p);
             hi[0] = w.x; hi[1] = w.y;
         }
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) hi[i] = 0;
+        for (int i = 0; i < kLen / 2; ++i) hi[i] = 0;
     }
 };
-template <int kPairs>
-struct Fragment<float, kPairs> {
-    static constexpr bool kSplit = true;
-    uint32_t hi[kPairs], lo[kPairs];
+template <int kLen>
+struct Fragment<float, kLen> {
+    uint32_t hi[kLen], lo[kLen];
+    __device__ __forceinline__ void set(int i, float v) {
+        hi[i] = ptx::tf32_rna_bits(v);
+        lo[i] = ptx::tf32_rna_bits(v - __uint_as_float(hi[i]));
+    }
     __device__ __forceinline__ void load(const float* p) {
 #pragma unroll
-        for (int i = 0; i < kPairs / 2; ++i) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
-            ptx::split_bf16x2(v.x, v.y, hi[2 * i], lo[2 * i]);
-            ptx::split_bf16x2(v.z, v.w, hi[2 * i + 1], lo[2 * i + 1]);
+        for (int i = 0; i < kLen / 4; ++i) {
+            const float4 v = reinterpret_cast<const float4*>(p)[i];
+            set(4 * i, v.x); set(4 * i + 1, v.y); set(4 * i + 2, v.z); set(4 * i + 3, v.w);
         }
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) hi[i] = lo[i] = 0;
+        for (int i = 0; i < kLen; ++i) hi[i] = lo[i] = 0;
     }
 };
+// v as the operand that meets T's: split in the parts that T's products want
+template <typename T, int kLen>
+struct SplitFragment;
+template <int kLen>
+struct SplitFragment<__nv_bfloat16, kLen> {
+    uint32_t hi[kLen / 2], lo[kLen / 2];
+    __device__ __forceinline__ void set(const float (&v)[kLen]) {
+#pragma unroll
+        for (int i = 0; i < kLen / 2; ++i) ptx::split_bf16x2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
+    }
+};
+template <int kLen>
+struct SplitFragment<float, kLen> : Fragment<float, kLen> {
+    __device__ __forceinline__ void set(const float (&v)[kLen]) {
+#pragma unroll
+        for (int i = 0; i < kLen; ++i) Fragment<float, kLen>::set(i, v[i]);
+    }
+};
+
+// c[n] += a b[n] over kLen consecutive contraction indices per lane, n = 0 ... kN - 1; rows g and g + 8 of the left operand.
+// Neighbouring instructions add into different accumulators: one that waits for its predecessor's takes four times as long.
+template <int kLen, int kN>
+__device__ __forceinline__ void multiply(float (*c)[4], const Fragment<__nv_bfloat16, kLen>& a0,
+                                         const Fragment<__nv_bfloat16, kLen>& a1, const Fragment<__nv_bfloat16, kLen> (&b)[kN]) {
+#pragma unroll
+    for (int s = 0; s < kLen / 2; s += 2)
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma16816(c[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b[n].hi[s], b[n].hi[s + 1]);
+}
+template <int kLen, int kN>
+__device__ __forceinline__ void multiply(float (*c)[4], const SplitFragment<__nv_bfloat16, kLen>& a0,
+                                         const SplitFragment<__nv_bfloat16, kLen>& a1, const Fragment<__nv_bfloat16, kLen> (&b)[kN]) {
+#pragma unroll
+    for (int s = 0; s < kLen / 2; s += 2) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma16816(c[n], a0.lo[s], a1.lo[s], a0.lo[s + 1], a1.lo[s + 1], b[n].hi[s], b[n].hi[s + 1]);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma16816(c[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b[n].hi[s], b[n].hi[s + 1]);
+    }
+}
+template <int kLen, int kN>
+__device__ __forceinline__ void multiply(float (*c)[4], const Fragment<float, kLen>& a0, const Fragment<float, kLen>& a1,
+                                         const Fragment<float, kLen> (&b)[kN]) {
+#pragma unroll
+    for (int s = 0; s < kLen; s += 2) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma1688(c[n], a0.lo[s], a1.lo[s], a0.lo[s + 1], a1.lo[s + 1], b[n].hi[s], b[n].hi[s + 1]);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma1688(c[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b[n].lo[s], b[n].lo[s + 1]);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma1688(c[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b[n].hi[s], b[n].hi[s + 1]);
+    }
+}
+template <typename T>
+constexpr int kGroup = sizeof(T) == 2 ? 4 : 2;  // fragments of the right operand held at a time
+
+// a fragment from shared memory, its 16-byte pieces `pitch` bytes apart
+__device__ __forceinline__ void load_pieces(Fragment<__nv_bfloat16, 8>& f, const uint8_t* p, int) {
+    f.load(reinterpret_cast<const __nv_bfloat16*>(p));
+}
+__device__ __forceinline__ void load_pieces(Fragment<__nv_bfloat16, 4>& f, const uint8_t* p, int) {
+    f.load(reinterpret_cast<const __nv_bfloat16*>(p));
+}
+template <int kLen>
+__device__ __forceinline__ void load_pieces(Fragment<float, kLen>& f, const uint8_t* p, int pitch) {
+#pragma unroll
+    for (int i = 0; i < kLen / 4; ++i) {
+        const float4 v = *reinterpret_cast<const float4*>(p + i * pitch);
+        f.set(4 * i, v.x); f.set(4 * i + 1, v.y); f.set(4 * i + 2, v.z); f.set(4 * i + 3, v.w);
+    }
+}
 
 // The adapter of token t, or kNone.  Offsets and ids come from the device unchecked: whatever they hold, the search stays
 // inside the arrays and ends, and an id outside [0, count) counts as none.
@@ -92,6 +177,7 @@ struct Units {
     int64_t per_part;   // features of a part, a multiple of 32
 };
 
+// ------------------------------------------------------------------------------------------------ a warp on its own
 // v[split][t][0 .. rank) = sum over the split's input features of x[t] D_a^T
 template <typename T, int kRank>  // kRank rows of D at a time: 16, 32 or 64
 __global__ void __launch_bounds__(32 * kWarps)
@@ -121,21 +207,15 @@ shrink_kernel(AdapterCall p, Units units) {
             for (int n = 0; n < kRank / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 #pragma unroll 2
             for (int64_t k = k0 + q * 8; k < k1; k += kStep) {
-                Fragment<T, 4> a0, a1;
+                Fragment<T, 8> a0, a1;
                 if (live0) a0.load(x + (t0 + g) * p.inner + k); else a0.clear();
                 if (live1) a1.load(x + (t0 + g + 8) * p.inner + k); else a1.clear();
 #pragma unroll
-                for (int n = 0; n < kRank / 8; ++n) {
-                    Fragment<T, 4> b;
-                    b.load(down + (int64_t)(n * 8 + g) * p.inner + k);
+                for (int n0 = 0; n0 < kRank / 8; n0 += 2) {
+                    Fragment<T, 8> b[2];
 #pragma unroll
-                    for (int s = 0; s < 4; s += 2) {
-                        mma16816(acc[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b.hi[s], b.hi[s + 1]);
-                        if constexpr (Fragment<T, 4>::kSplit) {
-                            mma16816(acc[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b.lo[s], b.lo[s + 1]);
-                            mma16816(acc[n], a0.lo[s], a1.lo[s], a0.lo[s + 1], a1.lo[s + 1], b.hi[s], b.hi[s + 1]);
-                        }
-                    }
+                    for (int n = 0; n < 2; ++n) b[n].load(down + (int64_t)((n0 + n) * 8 + g) * p.inner + k);
+                    multiply<8, 2>(acc + n0, a0, a1, b);
                 }
             }
             float* v = p.workspace + (part * p.tokens + t0) * p.rank + r0 + 2 * q;
@@ -149,25 +229,26 @@ shrink_kernel(AdapterCall p, Units units) {
     }
 }
 
-// the values of v that a lane holds as an operand: kPairs pairs of a row, summed over the splits, scaled, split in two
-template <int kPairs>
+// the values of v that a lane holds as an operand: kLen of token t from r on, summed over the splits and scaled
+template <typename T, int kLen>
 __device__ __forceinline__ void load_v(const AdapterCall& p, int64_t splits, int64_t t, int64_t r, float scale, bool wanted,
-                                       uint32_t (&hi)[kPairs], uint32_t (&lo)[kPairs]) {
-    float v[2 * kPairs];
+                                       SplitFragment<T, kLen>& f) {
+    float v[kLen];
 #pragma unroll
-    for (int i = 0; i < 2 * kPairs; ++i) v[i] = 0.f;
+    for (int i = 0; i < kLen; ++i) v[i] = 0.f;
     if (wanted) {
         for (int64_t s = 0; s < splits; ++s) {
             const float4* src = reinterpret_cast<const float4*>(p.workspace + (s * p.tokens + t) * p.rank + r);
 #pragma unroll
-            for (int i = 0; i < kPairs / 2; ++i) {
+            for (int i = 0; i < kLen / 4; ++i) {
                 const float4 w = src[i];
                 v[4 * i] += w.x; v[4 * i + 1] += w.y; v[4 * i + 2] += w.z; v[4 * i + 3] += w.w;
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) ptx::split_bf16x2(v[2 * i] * scale, v[2 * i + 1] * scale, hi[i], lo[i]);
+    for (int i = 0; i < kLen; ++i) v[i] *= scale;
+    f.set(v);
 }
 
 template <typename O>
@@ -185,8 +266,8 @@ __device__ __forceinline__ void add_base_and_store(const AdapterCall& p, int64_t
 template <typename T, typename O, int kRank>
 __global__ void __launch_bounds__(32 * kWarps)
 expand_kernel(AdapterCall p, Units units, int64_t splits) {
-    constexpr int kPairs = kRank == 16 ? 2 : 4;          // a lane's pairs of one load: 16 or 32 of the rank per warp load
-    constexpr int kLoads = kRank / (8 * kPairs);
+    constexpr int kLen = kRank == 16 ? 4 : 8;            // a lane's values of one load: 16 or 32 of the rank per warp load
+    constexpr int kLoads = kRank / (4 * kLen);
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (unit >= units.tiles * units.parts * units.subs) return;
@@ -216,13 +297,13 @@ expand_kernel(AdapterCall p, Units units, int64_t splits) {
         const bool row0 = ((rows >> g) & 1u) != 0, row1 = ((rows >> (g + 8)) & 1u) != 0;
         const float scale = __ldg(p.scaling + id);
         const T* up = static_cast<const T*>(p.up) + (int64_t)id * p.outer * p.rank;
-        uint32_t hi0[kLoads][kPairs], lo0[kLoads][kPairs], hi1[kLoads][kPairs], lo1[kLoads][kPairs];
+        SplitFragment<T, kLen> v0[kLoads], v1[kLoads];
         auto load_rank = [&](int64_t r0) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int64_t r = r0 + i * 8 * kPairs + q * 2 * kPairs;
-                load_v<kPairs>(p, splits, t0 + g, r, scale, row0, hi0[i], lo0[i]);
-                load_v<kPairs>(p, splits, t0 + g + 8, r, scale, row1, hi1[i], lo1[i]);
+                const int64_t r = r0 + (i * 4 + q) * kLen;
+                load_v<T, kLen>(p, splits, t0 + g, r, scale, row0, v0[i]);
+                load_v<T, kLen>(p, splits, t0 + g + 8, r, scale, row1, v1[i]);
             }
         };
         if (p.rank == kRank) load_rank(0);
@@ -233,21 +314,17 @@ expand_kernel(AdapterCall p, Units units, int64_t splits) {
             for (int64_t r0 = 0; r0 < p.rank; r0 += kRank) {
                 if (p.rank != kRank) load_rank(r0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t col = n + (g >> 1) * 8 + j * 2 + (g & 1);
+                for (int j0 = 0; j0 < 4; j0 += kGroup<T>)
 #pragma unroll
                     for (int i = 0; i < kLoads; ++i) {
-                        Fragment<T, kPairs> b;
-                        b.load(up + col * p.rank + r0 + i * 8 * kPairs + q * 2 * kPairs);
+                        Fragment<T, kLen> b[kGroup<T>];
 #pragma unroll
-                        for (int s = 0; s < kPairs; s += 2) {
-                            mma16816(acc[j], hi0[i][s], hi1[i][s], hi0[i][s + 1], hi1[i][s + 1], b.hi[s], b.hi[s + 1]);
-                            mma16816(acc[j], lo0[i][s], lo1[i][s], lo0[i][s + 1], lo1[i][s + 1], b.hi[s], b.hi[s + 1]);
-                            if constexpr (Fragment<T, kPairs>::kSplit)
-                                mma16816(acc[j], hi0[i][s], hi1[i][s], hi0[i][s + 1], hi1[i][s + 1], b.lo[s], b.lo[s + 1]);
+                        for (int j = 0; j < kGroup<T>; ++j) {
+                            const int64_t col = n + (g >> 1) * 8 + (j0 + j) * 2 + (g & 1);
+                            b[j].load(up + col * p.rank + r0 + (i * 4 + q) * kLen);
                         }
+                        multiply<kLen, kGroup<T>>(acc + j0, v0[i], v1[i], b);
                     }
-                }
             }
             if (row0) {
                 float v[8] = {acc[0][0], acc[0][1], acc[1][0], acc[1][1], acc[2][0], acc[2][1], acc[3][0], acc[3][1]};
@@ -261,47 +338,390 @@ expand_kernel(AdapterCall p, Units units, int64_t splits) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------- a CTA on 128 tokens
+constexpr int kTileTokens = 128, kTileWarps = 8, kTileThreads = 32 * kTileWarps;
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
+
+// The adapters of a CTA's tokens, in the order of their first token.  All threads call it alike.
+struct TileAdapters {
+    int* ids;          // shared: [128] adapter of each token
+    uint32_t* words;   // shared: [4] tokens not yet served
+    __device__ __forceinline__ void find(const AdapterCall& p, int64_t t0) {
+        const int i = threadIdx.x;
+        if (i < kTileTokens) {
+            const int id = adapter_of(t0 + i, p.tokens, p.offsets, p.ids, (int)p.requests, (int)p.count);
+            ids[i] = id;
+            const uint32_t w = __ballot_sync(0xffffffffu, id != kNone);
+            if ((i & 31) == 0) words[i >> 5] = w;
+        }
+        __syncthreads();
+    }
+    // the next adapter, or kNone; `rows`: bit r set where row r (of 16) of the calling thread's warp uses it
+    __device__ __forceinline__ int next(uint32_t& rows) {
+        int id = kNone;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t left = words[w];
+            if (id == kNone && left != 0) id = ids[w * 32 + __ffs(left) - 1];
+        }
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        rows = id == kNone ? 0u : __ballot_sync(0xffffffffu, lane < 16 && ids[warp * 16 + (lane & 15)] == id);
+        __syncthreads();  // everybody has read the words
+        if (id != kNone && threadIdx.x < kTileTokens) {
+            const uint32_t served = __ballot_sync(0xffffffffu, ids[threadIdx.x] == id);
+            if (lane == 0) words[warp] &= ~served;
+        }
+        __syncthreads();
+        return id;
+    }
+};
+
+// Shrink: a stage of the ring holds 128 bytes of k of the tile's tokens -- every lane copies the pieces that it will read
+// itself -- and of kRank rows of D, shared by the warps (16-byte piece c of row r at c ^ 4 (r mod 2): the two rows of a
+// quarter-warp's load use different banks).
+template <typename T, int kRank>
+struct ShrinkTile {
+    static constexpr int kStepK = 128 / (int)sizeof(T);             // input features of a stage
+    static constexpr int kXBytes = kTileTokens * 128, kDBytes = kRank * 128;
+    static constexpr int kStage = kXBytes + kDBytes;
+    static constexpr int kStages = 4;
+    static constexpr int kTotal = kStages * kStage;
+};
+
+template <typename T, int kRank>
+__global__ void __launch_bounds__(kTileThreads, 2)
+shrink_tile_kernel(AdapterCall p, Units units) {
+    using S = ShrinkTile<T, kRank>;
+    constexpr int kPieceLen = 16 / (int)sizeof(T);    // values of a 16-byte piece
+    constexpr int kPieces = 8 / kPieceLen;            // pieces of a fragment
+    constexpr int kSteps = S::kStepK / kStep;         // 32-feature steps of a stage
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int ids[kTileTokens];
+    __shared__ uint32_t words[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    // the tile's adapters are dealt to `subs` CTAs; those that most tiles have work for come first
+    const int64_t tile = blockIdx.x % units.tiles, part = blockIdx.x / units.tiles % units.parts;
+    const int sub = (int)(blockIdx.x / units.tiles / units.parts);
+    const int64_t k0 = part * units.per_part, k1 = min(p.inner, k0 + units.per_part);
+    const int64_t t0 = tile * kTileTokens;
+    const int range = (int)(k1 - k0), stages = (range + S::kStepK - 1) / S::kStepK;
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
+    const T* x = static_cast<const T*>(p.x);
+    const int64_t row0 = min(t0 + warp * 16 + g, p.tokens - 1), row1 = min(t0 + warp * 16 + g + 8, p.tokens - 1);
+
+    TileAdapters adapters = {ids, words};
+    adapters.find(p, t0);
+    for (int turn = 0;; ++turn) {
+        uint32_t rows;
+        const int id = adapters.next(rows);
+        if (id == kNone) break;
+        if (turn % units.subs != sub) continue;
+        for (int64_t r0 = 0; r0 < p.rank; r0 += kRank) {
+            const T* down = static_cast<const T*>(p.down) + ((int64_t)id * p.rank + r0) * p.inner;
+            // what this thread copies into every stage: two rows of x, up to kDPieces pieces of D
+            const T* x0 = x + row0 * p.inner + k0 + q * 8;
+            const T* x1 = x + row1 * p.inner + k0 + q * 8;
+            const int dr = threadIdx.x >> 3, dc = threadIdx.x & 7;
+            const T* d0 = down + (int64_t)dr * p.inner + k0 + dc * kPieceLen;
+            const uint32_t d_to = S::kXBytes + dr * 128 + ((dc ^ ((dr & 1) << 2)) << 4);
+            auto issue = [&](int s) {
+                if (s < stages) {
+                    const uint32_t stage = base + (s % S::kStages) * S::kStage;
+                    const int k = s * S::kStepK, left = range - k;  // features behind the stage's first
+                    if (rows != 0) {
+                        const uint32_t to = stage + threadIdx.x * 16;
+#pragma unroll
+                        for (int i = 0; i < kSteps; ++i)
+                            if (i * kStep < left) {
+#pragma unroll
+                                for (int c = 0; c < kPieces; ++c) {
+                                    copy16(to + (i * kPieces + c) * 2 * kTileThreads * 16, x0 + k + i * kStep + c * kPieceLen);
+                                    copy16(to + ((i * kPieces + c) * 2 + 1) * kTileThreads * 16, x1 + k + i * kStep + c * kPieceLen);
+                                }
+                            }
+                    }
+                    if (dc * kPieceLen < left) {
+#pragma unroll
+                        for (int j = 0; j < (kRank * 8 + kTileThreads - 1) / kTileThreads; ++j)
+                            if (j * 32 + dr < kRank) copy16(stage + d_to + j * 32 * 128, d0 + (int64_t)j * 32 * p.inner + k);
+                    }
+                }
+                commit_copies();
+            };
+            float acc[kRank / 8][4];
+#pragma unroll
+            for (int n = 0; n < kRank / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll
+            for (int s = 0; s < S::kStages - 1; ++s) issue(s);
+            for (int s = 0; s < stages; ++s) {
+                wait_copies<S::kStages - 2>();
+                __syncthreads();  // the stage has arrived for everybody, and the one before has been read by everybody
+                issue(s + S::kStages - 1);
+                if (rows == 0) continue;
+                const uint8_t* stage = smem + (s % S::kStages) * S::kStage;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    if (s * S::kStepK + i * kStep >= range) break;
+                    Fragment<T, 8> a0, a1;
+                    load_pieces(a0, stage + (i * kPieces * 2 * kTileThreads + threadIdx.x) * 16, 2 * kTileThreads * 16);
+                    load_pieces(a1, stage + (i * kPieces * 2 * kTileThreads + kTileThreads + threadIdx.x) * 16, 2 * kTileThreads * 16);
+#pragma unroll
+                    for (int n0 = 0; n0 < kRank / 8; n0 += 2) {
+                        Fragment<T, 8> b[2];
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+                            load_pieces(b[n], stage + S::kXBytes + ((n0 + n) * 8 + g) * 128 + ((((i * 4 + q) * kPieces) ^ ((g & 1) << 2)) << 4), 16);
+                        multiply<8, 2>(acc + n0, a0, a1, b);
+                    }
+                }
+            }
+            wait_copies<0>();
+            __syncthreads();  // the ring is free for the next round
+            float* v = p.workspace + (part * p.tokens + t0 + warp * 16) * p.rank + r0 + 2 * q;
+#pragma unroll
+            for (int n = 0; n < kRank / 8; ++n) {
+                if ((rows >> g) & 1u) *reinterpret_cast<float2*>(v + g * p.rank + n * 8) = make_float2(acc[n][0], acc[n][1]);
+                if ((rows >> (g + 8)) & 1u)
+                    *reinterpret_cast<float2*>(v + (g + 8) * p.rank + n * 8) = make_float2(acc[n][2], acc[n][3]);
+            }
+        }
+    }
+}
+
+// Expand: the ring passes kExpandCols columns of U_a (rows of the stored matrix) at a time to the CTA's warps, and to every
+// lane the pieces of the base that it will add to.
+constexpr int kExpandCols = 64, kExpandStages = 3;
+template <typename T, typename O, int kRank>
+struct ExpandTile {
+    static constexpr int kUBytes = kExpandCols * kRank * (int)sizeof(T);
+    static constexpr int kBaseBytes = kTileTokens * kExpandCols * (int)sizeof(O);
+    static constexpr int kStage = kUBytes + kBaseBytes;
+    static constexpr int kTotal = kExpandStages * kStage;
+};
+
+template <typename T, typename O, int kRank>
+__global__ void __launch_bounds__(kTileThreads, 2)
+expand_tile_kernel(AdapterCall p, Units units, int64_t splits) {
+    constexpr int kLen = kRank == 16 ? 4 : 8;
+    constexpr int kLoads = kRank / (4 * kLen);
+    constexpr int kRowBytes = kRank * (int)sizeof(T);
+    constexpr int kRowPieces = kRowBytes / 16;
+    constexpr int kSwizzle = kRowPieces >= 8 ? 4 : 0;  // shorter rows: two neighbours share a 128-byte line as they lie
+    using S = ExpandTile<T, O, kRank>;
+    constexpr int kStage = S::kStage;
+    constexpr int kBaseLen = 16 / (int)sizeof(O), kBasePieces = 8 / kBaseLen;  // of eight consecutive outputs
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int ids[kTileTokens];
+    __shared__ uint32_t words[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    // the tile's adapters are dealt to `subs` CTAs; those that most tiles have work for come first
+    const int64_t tile = blockIdx.x % units.tiles, part = blockIdx.x / units.tiles % units.parts;
+    const int sub = (int)(blockIdx.x / units.tiles / units.parts);
+    const int64_t n0 = part * units.per_part, n1 = min(p.outer, n0 + units.per_part);
+    const int64_t t0 = tile * kTileTokens;
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
+
+    TileAdapters adapters = {ids, words};
+    adapters.find(p, t0);
+    if (sub == 0 && p.base != p.out) {  // tokens without an adapter keep their base
+        for (int row = warp; row < kTileTokens; row += kTileWarps) {
+            if (ids[row] != kNone || t0 + row >= p.tokens) continue;
+            for (int64_t n = n0 + lane * 8; n < n1; n += 256) {
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                add_base_and_store<O>(p, t0 + row, n, v);
+            }
+        }
+    }
+    const int chunks = (int)((n1 - n0 + kExpandCols - 1) / kExpandCols);
+    const int rounds = (int)(p.rank / kRank);  // a chunk's columns pass in `rounds` pieces of the rank
+    for (int turn = 0;; ++turn) {
+        uint32_t rows;
+        const int id = adapters.next(rows);
+        if (id == kNone) break;
+        if (turn % units.subs != sub) continue;
+        const bool row0 = ((rows >> g) & 1u) != 0, row1 = ((rows >> (g + 8)) & 1u) != 0;
+        const int64_t tok0 = t0 + warp * 16 + g, tok1 = tok0 + 8;
+        const float scale = __ldg(p.scaling + id);
+        const T* up = static_cast<const T*>(p.up) + (int64_t)id * p.outer * p.rank;
+        // what this thread copies into every stage: kUCopies pieces of U, and of the base what it adds to
+        constexpr int kUCopies = (kExpandCols * kRowPieces + kTileThreads - 1) / kTileThreads, kUStep = kTileThreads / kRowPieces;
+        const int ucol = threadIdx.x / kRowPieces, uc = threadIdx.x % kRowPieces;
+        const T* u0 = up + (n0 + ucol) * p.rank + uc * (16 / (int)sizeof(T));
+        const uint32_t u_to = ucol * kRowBytes + ((uc ^ ((ucol & 1) * kSwizzle)) << 4);
+        static_assert(kUStep % 2 == 0, "a thread's columns have one parity");
+        const O* base0 = static_cast<const O*>(p.base) + tok0 * p.outer + n0 + q * 8;
+        const O* base1 = static_cast<const O*>(p.base) + tok1 * p.outer + n0 + q * 8;
+        const bool copy0 = row0 && p.base != nullptr, copy1 = row1 && p.base != nullptr;
+        auto issue = [&](int s) {
+            if (s < chunks * rounds) {
+                const uint32_t stage = base + (s % kExpandStages) * kStage;
+                const int chunk = rounds == 1 ? s : s / rounds, round = rounds == 1 ? 0 : s % rounds;
+                const int n = chunk * kExpandCols, left = (int)(n1 - n0) - n;
+                const T* u = u0 + n * p.rank + round * kRank;
+#pragma unroll
+                for (int j = 0; j < kUCopies; ++j)
+                    if (j * kUStep + ucol < kExpandCols && j * kUStep + ucol < left)
+                        copy16(stage + u_to + j * kUStep * kRowBytes, u + (int64_t)j * kUStep * p.rank);
+                if (round == rounds - 1) {
+                    const uint32_t to = stage + S::kUBytes + threadIdx.x * 16;
+#pragma unroll
+                    for (int h = 0; h < kExpandCols / 32; ++h)
+                        if (h * 32 < left) {
+#pragma unroll
+                            for (int e = 0; e < kBasePieces; ++e) {
+                                if (copy0) copy16(to + (h * 2 * kBasePieces + e) * kTileThreads * 16, base0 + n + h * 32 + e * kBaseLen);
+                                if (copy1) copy16(to + ((h * 2 + 1) * kBasePieces + e) * kTileThreads * 16, base1 + n + h * 32 + e * kBaseLen);
+                            }
+                        }
+                }
+            }
+            commit_copies();
+        };
+        SplitFragment<T, kLen> v0[kLoads], v1[kLoads];
+        auto load_rank = [&](int64_t r0) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int64_t r = r0 + (i * 4 + q) * kLen;
+                load_v<T, kLen>(p, splits, tok0, r, scale, row0, v0[i]);
+                load_v<T, kLen>(p, splits, tok1, r, scale, row1, v1[i]);
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < kExpandStages - 1; ++s) issue(s);
+        if (rounds == 1 && rows != 0) load_rank(0);
+        float acc[kExpandCols / 8][4];
+        for (int s = 0; s < chunks * rounds; ++s) {
+            const int round = s % rounds;
+            const int64_t n = n0 + (int64_t)(s / rounds) * kExpandCols;
+            wait_copies<kExpandStages - 2>();
+            __syncthreads();
+            issue(s + kExpandStages - 1);
+            if (rows == 0) continue;
+            if (rounds > 1) load_rank((int64_t)round * kRank);
+            if (round == 0) {
+#pragma unroll
+                for (int j = 0; j < kExpandCols / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+            }
+            const uint8_t* stage = smem + (s % kExpandStages) * kStage;
+#pragma unroll
+            for (int j0 = 0; j0 < kExpandCols / 8; j0 += kGroup<T>)
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    Fragment<T, kLen> b[kGroup<T>];
+#pragma unroll
+                    for (int j = 0; j < kGroup<T>; ++j) {
+                        const int col = (j0 + j) / 4 * 32 + (g >> 1) * 8 + (j0 + j) % 4 * 2 + (g & 1);
+                        const int c = (i * 4 + q) * kLen * (int)sizeof(T);  // byte in the row
+                        load_pieces(b[j], stage + col * kRowBytes + (c ^ ((g & 1) * kSwizzle * 16)), 16);
+                    }
+                    multiply<kLen, kGroup<T>>(acc + j0, v0[i], v1[i], b);
+                }
+            if (round != rounds - 1) continue;
+#pragma unroll
+            for (int h = 0; h < kExpandCols / 32; ++h) {
+                const int64_t c = n + h * 32 + q * 8;
+                if (c >= n1) break;
+                const uint8_t* from = stage + S::kUBytes + (h * 2 * kBasePieces * kTileThreads + threadIdx.x) * 16;
+#pragma unroll
+                for (int second = 0; second < 2; ++second) {
+                    if (second ? !row1 : !row0) continue;
+                    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    if (p.base != nullptr) {
+                        Raw8<O> b;
+                        b.load_pieces(from + second * kBasePieces * kTileThreads * 16, kTileThreads * 16);
+                        b.unpack(v);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += acc[h * 4 + (e >> 1)][2 * second + (e & 1)];
+                    store8(static_cast<O*>(p.out) + (second ? tok1 : tok0) * p.outer + c, v);
+                }
+            }
+        }
+        wait_copies<0>();
+        __syncthreads();  // the ring is free for the next adapter
+    }
+}
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 constexpr int64_t kWantedWarps = 148 * 8;
 
-// How the input features are cut: enough warps to fill the GPU, at least 128 features each, at most 16 partial sums.
-Units shrink_units(int64_t tokens, int64_t inner) {
+// Prompts go by tiles of 128 tokens, short requests by warps of 16: TILES_NOTE
+bool by_tiles(int64_t tokens, int64_t requests) { return tokens >= 256 && tokens >= 32 * requests; }
+
+// How the input features are cut: enough warps (or CTAs) to fill the GPU, at least 128 (256) features each, at most 16
+// partial sums.
+Units shrink_units(int64_t tokens, int64_t inner, bool tiles) {
     Units u;
-    u.tiles = ceil_div(tokens, kTokens);
+    u.tiles = ceil_div(tokens, tiles ? kTileTokens : kTokens);
     u.subs = 1;
-    int64_t parts = ceil_div(kWantedWarps, u.tiles);
+    int64_t parts = tiles ? 148 / u.tiles : ceil_div(kWantedWarps, u.tiles);
     parts = parts < 16 ? parts : 16;
-    const int64_t most = ceil_div(inner, 128);
+    const int64_t most = ceil_div(inner, tiles ? 256 : 128);
     parts = parts < most ? parts : most;
-    u.per_part = ceil_div(ceil_div(inner, parts), 32) * 32;
+    parts = parts < 1 ? 1 : parts;
+    u.per_part = ceil_div(ceil_div(inner, parts), 64) * 64;
     u.parts = ceil_div(inner, u.per_part);
     return u;
 }
 
-// Distinct adapters a tile may hold: as many as the requests that meet in it, on average.
-int sub_count(const AdapterCall& p) {
+// Distinct adapters a warp's 16 tokens may hold: as many as the requests that meet in it, on average.  A tile of 128
+// prompt tokens: 4, because a CTA that serves two adapters takes twice as long as its neighbours, and one without work is
+// gone at once.
+int sub_count(const AdapterCall& p, bool tiles) {
+    if (tiles) return p.requests < 4 ? (int)(p.requests > 1 ? p.requests : 1) : 4;
     const int64_t meet = ceil_div(kTokens * p.requests, p.tokens);
     int subs = 1;
     while (subs < meet && subs < kTokens) subs *= 2;
     return subs;
 }
 
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, bool (&ready)[64]) {  // per device; racing first calls set it twice
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (ready[dev]) return cudaSuccess;
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err == cudaSuccess) ready[dev] = true;
+    return err;
+}
+
 template <typename T, typename O, int kRank>
 cudaError_t launch(const AdapterCall& p, cudaStream_t stream) {
-    Units shrink = shrink_units(p.tokens, p.inner);
+    const bool tiles = by_tiles(p.tokens, p.requests);
+    Units shrink = shrink_units(p.tokens, p.inner, tiles);
     Units expand = shrink;
-    shrink.subs = expand.subs = sub_count(p);
-    int64_t parts = ceil_div(kWantedWarps * 2, expand.tiles * expand.subs);
-    const int64_t most = p.outer / 32;
+    shrink.subs = expand.subs = sub_count(p, tiles);
+    const int64_t unit = tiles ? kExpandCols : 32, most = ceil_div(p.outer, unit);
+    int64_t parts = tiles ? 2 * 148 / expand.tiles : ceil_div(kWantedWarps * 2, expand.tiles * expand.subs);
     parts = parts < most ? parts : most;
-    expand.per_part = ceil_div(most, parts) * 32;
+    parts = parts < 1 ? 1 : parts;
+    expand.per_part = ceil_div(most, parts) * unit;
     expand.parts = ceil_div(p.outer, expand.per_part);
-    const int64_t shrink_ctas = ceil_div(shrink.tiles * shrink.parts * shrink.subs, kWarps);
-    const int64_t expand_ctas = ceil_div(expand.tiles * expand.parts * expand.subs, kWarps);
+    const int64_t per_cta = tiles ? 1 : kWarps;
+    const int64_t shrink_ctas = ceil_div(shrink.tiles * shrink.parts * shrink.subs, per_cta);
+    const int64_t expand_ctas = ceil_div(expand.tiles * expand.parts * expand.subs, per_cta);
     if (shrink_ctas > 0x7fffffffll || expand_ctas > 0x7fffffffll) return cudaErrorInvalidValue;
-    shrink_kernel<T, kRank><<<(unsigned)shrink_ctas, 32 * kWarps, 0, stream>>>(p, shrink);
-    expand_kernel<T, O, kRank><<<(unsigned)expand_ctas, 32 * kWarps, 0, stream>>>(p, expand, shrink.parts);
+    if (tiles) {
+        constexpr int kShrinkBytes = ShrinkTile<T, kRank>::kTotal, kExpandBytes = ExpandTile<T, O, kRank>::kTotal;
+        static bool shrink_ready[64] = {false}, expand_ready[64] = {false};
+        cudaError_t err = allow_smem(shrink_tile_kernel<T, kRank>, kShrinkBytes, shrink_ready);
+        if (err == cudaSuccess) err = allow_smem(expand_tile_kernel<T, O, kRank>, kExpandBytes, expand_ready);
+        if (err != cudaSuccess) return err;
+        shrink_tile_kernel<T, kRank><<<(unsigned)shrink_ctas, kTileThreads, kShrinkBytes, stream>>>(p, shrink);
+        expand_tile_kernel<T, O, kRank><<<(unsigned)expand_ctas, kTileThreads, kExpandBytes, stream>>>(p, expand, shrink.parts);
+    } else {
+        shrink_kernel<T, kRank><<<(unsigned)shrink_ctas, 32 * kWarps, 0, stream>>>(p, shrink);
+        expand_kernel<T, O, kRank><<<(unsigned)expand_ctas, 32 * kWarps, 0, stream>>>(p, expand, shrink.parts);
+    }
     return cudaGetLastError();
 }
 
@@ -317,7 +737,8 @@ cudaError_t by_rank(const AdapterCall& p, cudaStream_t stream) {
 
 int64_t adapters_workspace_bytes(int64_t tokens, int64_t inner, int64_t rank) {
     if (tokens == 0) return 0;
-    return shrink_units(tokens, inner).parts * tokens * rank * (int64_t)sizeof(float);
+    const int64_t a = shrink_units(tokens, inner, false).parts, b = shrink_units(tokens, inner, true).parts;
+    return (a > b ? a : b) * tokens * rank * (int64_t)sizeof(float);
 }
 
 cudaError_t launch_adapters(const AdapterCall& p, bool in_bf16, bool out_bf16, cudaStream_t stream) {

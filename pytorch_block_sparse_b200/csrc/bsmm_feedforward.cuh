@@ -56,6 +56,10 @@ struct Raw8<float> {
         a = *reinterpret_cast<const float4*>(p);
         b = *reinterpret_cast<const float4*>(p + 4);
     }
+    __device__ __forceinline__ void load_pieces(const uint8_t* p, int pitch) {  // 16-byte pieces `pitch` bytes apart
+        a = *reinterpret_cast<const float4*>(p);
+        b = *reinterpret_cast<const float4*>(p + pitch);
+    }
     __device__ __forceinline__ void unpack(float (&v)[8]) const {
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
         v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -65,6 +69,7 @@ template <>
 struct Raw8<__nv_bfloat16> {
     uint4 a;
     __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void load_pieces(const uint8_t* p, int) { a = *reinterpret_cast<const uint4*>(p); }
     __device__ __forceinline__ void unpack(float (&v)[8]) const { unpack8(a, v); }
 };
 

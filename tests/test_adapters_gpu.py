@@ -73,8 +73,11 @@ MIXES = {
 @pytest.mark.parametrize("types", ["fp32", "bf16", "bf16 in fp32"])
 @pytest.mark.parametrize("sizes", [(32, 32, 1), (96, 160, 8), (1056, 544, 16), (256, 96, 24), (160, 2080, 64), (64, 64, 100)])
 def test_mixes_ranks_and_types(mix, types, sizes):
+    run_mix(*MIXES[mix], types, sizes)
+
+
+def run_mix(lengths, ids, types, sizes):
     inner, outer, rank = sizes
-    lengths, ids = MIXES[mix]
     dtype = torch.float32 if types == "fp32" else torch.bfloat16
     out_dtype = torch.bfloat16 if types == "bf16" else torch.float32
     ad, weights = make(inner, outer, 5, rank, dtype, seed=3)
@@ -90,6 +93,21 @@ def test_mixes_ranks_and_types(mix, types, sizes):
         assert torch.equal(again, got)  # in place, and the same bits a second time
         alone = ad(x.cuda(), requests, dtype=out_dtype)
         check(alone, x, lengths, ids, weights, torch.zeros_like(base), dtype, inner, rank)
+
+
+PROMPTS = {  # long enough for the form that owns 128 tokens at a time
+    "one": ([256], [1]),
+    "odd": ([257, 130, 0, 1, 3, 129], [0, 3, 1, 2, None, 4]),
+    "many adapters in a tile": ([500, 5, 1, 7, 2, 30, 1, 60], [0, 1, 2, 3, 4, 0, 1, 2]),
+    "none but one": ([300, 20, 300], [None, 4, None]),
+}
+
+
+@pytest.mark.parametrize("mix", PROMPTS)
+@pytest.mark.parametrize("types", ["fp32", "bf16", "bf16 in fp32"])
+@pytest.mark.parametrize("sizes", [(32, 32, 1), (96, 160, 16), (1056, 544, 24), (544, 2080, 64), (64, 96, 200)])
+def test_prompts(mix, types, sizes):
+    run_mix(*PROMPTS[mix], types, sizes)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -115,6 +133,13 @@ def test_tokens_outside_every_request_keep_their_base():
         check(got[3:40], x[3:40], [7, 30], [0, 1], weights, base[3:40], torch.float32, 64, 16)
         alone = ad(x.cuda(), requests).cpu()
         assert (alone[:3] == 0).all() and (alone[40:] == 0).all()
+        # the same for long prompts
+        xl, bl = randn((600, 64), 3), randn((600, 64), 4)
+        xl[:3], xl[570:] = float("inf"), float("nan")
+        long = AdapterRequests(torch.tensor([3, 300, 570], dtype=torch.int32, device="cuda"), torch.tensor([1, 0], dtype=torch.int32, device="cuda"))
+        got = ad(xl.cuda(), long, base=bl.cuda()).cpu()
+        assert torch.equal(got[:3], bl[:3]) and torch.equal(got[570:], bl[570:])
+        check(got[3:570], xl[3:570], [297, 270], [1, 0], weights, bl[3:570], torch.float32, 64, 16)
         # a token's NaN stays its own
         x2 = randn((50, 64), 1)
         x2[20] = float("nan")
