@@ -17,6 +17,7 @@
 // Arithmetic.  fp32 tensors: both operands are split into tf32 hi + lo parts and three products are added (about 2^-21
 // relative per term); bf16 tensors: x D is one exact product, v is split into bf16 hi + lo (its rounding to one bf16 would
 // cost as much as the output's own).
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include "bsmm_feedforward.cuh"
@@ -24,6 +25,8 @@
 
 namespace bsmm {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kTokens = 16;       // tokens of a warp
 constexpr int kWarps = 4;         // warps of a CTA, each on its own
@@ -155,6 +158,12 @@ __device__ __forceinline__ void load_pieces(Fragment<float, kLen>& f, const uint
     }
 }
 
+// The expand kernel is launched while the shrink kernel still runs (programmatic dependent launch): what it does before
+// this wait -- finding its work, the first loads of U and of the base -- overlaps the other's tail.  Every thread waits before
+// it leaves, so that the expand grid never completes before the shrink grid.
+__device__ __forceinline__ void wait_for_shrink() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_expand_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // The adapter of token t, or kNone.  Offsets and ids come from the device unchecked: whatever they hold, the search stays
 // inside the arrays and ends, and an id outside [0, count) counts as none.
 __device__ __forceinline__ int adapter_of(int64_t t, int64_t tokens, const int32_t* __restrict__ offsets,
@@ -184,6 +193,7 @@ __global__ void __launch_bounds__(32 * kWarps)
 shrink_kernel(AdapterCall p, Units units) {
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    let_expand_start();
     if (unit >= units.tiles * units.parts * units.subs) return;
     const int64_t tile = unit % units.tiles, rest = unit / units.tiles;
     const int sub = (int)(rest % units.subs);
@@ -270,7 +280,10 @@ expand_kernel(AdapterCall p, Units units, int64_t splits) {
     constexpr int kLoads = kRank / (4 * kLen);
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (unit >= units.tiles * units.parts * units.subs) return;
+    if (unit >= units.tiles * units.parts * units.subs) {
+        wait_for_shrink();
+        return;
+    }
     const int64_t tile = unit % units.tiles, rest = unit / units.tiles;
     const int sub = (int)(rest % units.subs);
     const int64_t part = rest / units.subs;
@@ -289,6 +302,7 @@ expand_kernel(AdapterCall p, Units units, int64_t splits) {
             }
         }
     }
+    wait_for_shrink();
     for (int turn = 0; todo != 0; ++turn) {
         const int id = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
         const uint32_t rows = __ballot_sync(0xffffffffu, mine == id);
@@ -348,43 +362,49 @@ __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_
 template <int kPending>
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
 
-// The adapters of a CTA's tokens, in the order of their first token.  All threads call it alike.
-struct TileAdapters {
-    int* ids;          // shared: [128] adapter of each token
-    uint32_t* words;   // shared: [4] tokens not yet served
-    __device__ __forceinline__ void find(const AdapterCall& p, int64_t t0) {
-        const int i = threadIdx.x;
-        if (i < kTileTokens) {
-            const int id = adapter_of(t0 + i, p.tokens, p.offsets, p.ids, (int)p.requests, (int)p.count);
-            ids[i] = id;
-            const uint32_t w = __ballot_sync(0xffffffffu, id != kNone);
-            if ((i & 31) == 0) words[i >> 5] = w;
-        }
-        __syncthreads();
-    }
-    // the next adapter, or kNone; `rows`: bit r set where row r (of 16) of the calling thread's warp uses it
-    __device__ __forceinline__ int next(uint32_t& rows) {
-        int id = kNone;
+// Up to 128 tokens of one request.  The requests' tokens are cut into such tiles from each request's start; the tokens before
+// the first request and behind the last one count as requests without an adapter.
+struct Tile {
+    int first, rows, id;
+    // Each warp finds the tile by itself, 32 requests at a time.  False: there are fewer tiles.
+    __device__ __forceinline__ bool find(const AdapterCall& p, int tile) {
+        const int lane = threadIdx.x & 31, requests = (int)p.requests, tokens = (int)p.tokens;
+        int before = 0;
+        for (int r0 = -1; r0 <= requests; r0 += 32) {
+            const int r = r0 + lane;
+            int start = 0, end = 0, adapter = kNone;
+            if (r <= requests) {
+                start = r < 0 ? 0 : min(max(__ldg(p.offsets + r), 0), tokens);
+                end = r == requests ? tokens : min(max(__ldg(p.offsets + r + 1), 0), tokens);
+                if (r >= 0 && r < requests) adapter = __ldg(p.ids + r);
+                if (adapter < 0 || adapter >= p.count) adapter = kNone;
+            }
+            const int tiles = (max(end - start, 0) + kTileTokens - 1) / kTileTokens;
+            int sum = tiles;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t left = words[w];
-            if (id == kNone && left != 0) id = ids[w * 32 + __ffs(left) - 1];
+            for (int o = 1; o < 32; o <<= 1) {
+                const int below = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += below;
+            }
+            const uint32_t reached = __ballot_sync(0xffffffffu, before + sum > tile);
+            if (reached != 0) {
+                const int src = __ffs(reached) - 1;
+                const int skipped = tile - before - __shfl_sync(0xffffffffu, sum - tiles, src);
+                first = __shfl_sync(0xffffffffu, start, src) + skipped * kTileTokens;
+                rows = min(kTileTokens, __shfl_sync(0xffffffffu, end, src) - first);
+                id = __shfl_sync(0xffffffffu, adapter, src);
+                return true;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
         }
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        rows = id == kNone ? 0u : __ballot_sync(0xffffffffu, lane < 16 && ids[warp * 16 + (lane & 15)] == id);
-        __syncthreads();  // everybody has read the words
-        if (id != kNone && threadIdx.x < kTileTokens) {
-            const uint32_t served = __ballot_sync(0xffffffffu, ids[threadIdx.x] == id);
-            if (lane == 0) words[warp] &= ~served;
-        }
-        __syncthreads();
-        return id;
+        return false;
     }
 };
 
 // Shrink: a stage of the ring holds 128 bytes of k of the tile's tokens -- every lane copies the pieces that it will read
 // itself -- and of kRank rows of D, shared by the warps (16-byte piece c of row r at c ^ 4 (r mod 2): the two rows of a
-// quarter-warp's load use different banks).
+// quarter-warp's load use different banks).  The CTAs of a cluster take a part of the input features each and add their sums
+// up through distributed shared memory, every one a share of the tokens, in the order of the parts.
 template <typename T, int kRank>
 struct ShrinkTile {
     static constexpr int kStepK = 128 / (int)sizeof(T);             // input features of a stage
@@ -392,6 +412,7 @@ struct ShrinkTile {
     static constexpr int kStage = kXBytes + kDBytes;
     static constexpr int kStages = 4;
     static constexpr int kTotal = kStages * kStage;
+    static_assert(kTotal >= kTileTokens * kRank * 4, "the sums reuse the ring");
 };
 
 template <typename T, int kRank>
@@ -401,251 +422,276 @@ shrink_tile_kernel(AdapterCall p, Units units) {
     constexpr int kPieceLen = 16 / (int)sizeof(T);    // values of a 16-byte piece
     constexpr int kPieces = 8 / kPieceLen;            // pieces of a fragment
     constexpr int kSteps = S::kStepK / kStep;         // 32-feature steps of a stage
+    constexpr int kN = kRank / 8 < kGroup<T> ? kRank / 8 : kGroup<T>;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int ids[kTileTokens];
-    __shared__ uint32_t words[4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    // the tile's adapters are dealt to `subs` CTAs; those that most tiles have work for come first
-    const int64_t tile = blockIdx.x % units.tiles, part = blockIdx.x / units.tiles % units.parts;
-    const int sub = (int)(blockIdx.x / units.tiles / units.parts);
-    const int64_t k0 = part * units.per_part, k1 = min(p.inner, k0 + units.per_part);
-    const int64_t t0 = tile * kTileTokens;
+    const int parts = (int)units.parts, part = (int)blockIdx.x % parts;
+    const int64_t k0 = min(p.inner, part * units.per_part), k1 = min(p.inner, k0 + units.per_part);
     const int range = (int)(k1 - k0), stages = (range + S::kStepK - 1) / S::kStepK;
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-    const T* x = static_cast<const T*>(p.x);
-    const int64_t row0 = min(t0 + warp * 16 + g, p.tokens - 1), row1 = min(t0 + warp * 16 + g + 8, p.tokens - 1);
+    let_expand_start();
+    Tile tile;
+    if (!tile.find(p, (int)blockIdx.x / parts) || tile.id == kNone) return;  // (the whole cluster alike)
 
-    TileAdapters adapters = {ids, words};
-    adapters.find(p, t0);
-    for (int turn = 0;; ++turn) {
-        uint32_t rows;
-        const int id = adapters.next(rows);
-        if (id == kNone) break;
-        if (turn % units.subs != sub) continue;
-        for (int64_t r0 = 0; r0 < p.rank; r0 += kRank) {
-            const T* down = static_cast<const T*>(p.down) + ((int64_t)id * p.rank + r0) * p.inner;
-            // what this thread copies into every stage: two rows of x, up to kDPieces pieces of D
-            const T* x0 = x + row0 * p.inner + k0 + q * 8;
-            const T* x1 = x + row1 * p.inner + k0 + q * 8;
-            const int dr = threadIdx.x >> 3, dc = threadIdx.x & 7;
-            const T* d0 = down + (int64_t)dr * p.inner + k0 + dc * kPieceLen;
-            const uint32_t d_to = S::kXBytes + dr * 128 + ((dc ^ ((dr & 1) << 2)) << 4);
-            auto issue = [&](int s) {
-                if (s < stages) {
-                    const uint32_t stage = base + (s % S::kStages) * S::kStage;
-                    const int k = s * S::kStepK, left = range - k;  // features behind the stage's first
-                    if (rows != 0) {
-                        const uint32_t to = stage + threadIdx.x * 16;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int last = tile.first + tile.rows - 1, t0 = tile.first + warp * 16 + g;
+    const bool busy = warp * 16 < tile.rows;
+    const T* x0 = static_cast<const T*>(p.x) + (int64_t)min(t0, last) * p.inner + k0 + q * 8;
+    const T* x1 = static_cast<const T*>(p.x) + (int64_t)min(t0 + 8, last) * p.inner + k0 + q * 8;
+    for (int64_t r0 = 0; r0 < p.rank; r0 += kRank) {
+        const int dr = threadIdx.x >> 3, dc = threadIdx.x & 7;
+        const T* d0 = static_cast<const T*>(p.down) + ((int64_t)tile.id * p.rank + r0 + dr) * p.inner + k0 + dc * kPieceLen;
+        const uint32_t d_to = S::kXBytes + dr * 128 + ((dc ^ ((dr & 1) << 2)) << 4);
+        auto issue = [&](int s) {
+            if (s < stages) {
+                const uint32_t stage = base + (s % S::kStages) * S::kStage;
+                const int k = s * S::kStepK, left = range - k;  // features behind the stage's first
+                if (busy) {
+                    const uint32_t to = stage + threadIdx.x * 16;
 #pragma unroll
-                        for (int i = 0; i < kSteps; ++i)
-                            if (i * kStep < left) {
+                    for (int i = 0; i < kSteps; ++i)
+                        if (i * kStep < left) {
 #pragma unroll
-                                for (int c = 0; c < kPieces; ++c) {
-                                    copy16(to + (i * kPieces + c) * 2 * kTileThreads * 16, x0 + k + i * kStep + c * kPieceLen);
-                                    copy16(to + ((i * kPieces + c) * 2 + 1) * kTileThreads * 16, x1 + k + i * kStep + c * kPieceLen);
-                                }
+                            for (int c = 0; c < kPieces; ++c) {
+                                copy16(to + (i * kPieces + c) * 2 * kTileThreads * 16, x0 + k + i * kStep + c * kPieceLen);
+                                copy16(to + ((i * kPieces + c) * 2 + 1) * kTileThreads * 16, x1 + k + i * kStep + c * kPieceLen);
                             }
-                    }
-                    if (dc * kPieceLen < left) {
-#pragma unroll
-                        for (int j = 0; j < (kRank * 8 + kTileThreads - 1) / kTileThreads; ++j)
-                            if (j * 32 + dr < kRank) copy16(stage + d_to + j * 32 * 128, d0 + (int64_t)j * 32 * p.inner + k);
-                    }
+                        }
                 }
-                commit_copies();
-            };
-            float acc[kRank / 8][4];
+                if (dc * kPieceLen < left) {
 #pragma unroll
-            for (int n = 0; n < kRank / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-#pragma unroll
-            for (int s = 0; s < S::kStages - 1; ++s) issue(s);
-            for (int s = 0; s < stages; ++s) {
-                wait_copies<S::kStages - 2>();
-                __syncthreads();  // the stage has arrived for everybody, and the one before has been read by everybody
-                issue(s + S::kStages - 1);
-                if (rows == 0) continue;
-                const uint8_t* stage = smem + (s % S::kStages) * S::kStage;
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    if (s * S::kStepK + i * kStep >= range) break;
-                    Fragment<T, 8> a0, a1;
-                    load_pieces(a0, stage + (i * kPieces * 2 * kTileThreads + threadIdx.x) * 16, 2 * kTileThreads * 16);
-                    load_pieces(a1, stage + (i * kPieces * 2 * kTileThreads + kTileThreads + threadIdx.x) * 16, 2 * kTileThreads * 16);
-#pragma unroll
-                    for (int n0 = 0; n0 < kRank / 8; n0 += 2) {
-                        Fragment<T, 8> b[2];
-#pragma unroll
-                        for (int n = 0; n < 2; ++n)
-                            load_pieces(b[n], stage + S::kXBytes + ((n0 + n) * 8 + g) * 128 + ((((i * 4 + q) * kPieces) ^ ((g & 1) << 2)) << 4), 16);
-                        multiply<8, 2>(acc + n0, a0, a1, b);
-                    }
+                    for (int j = 0; j < (kRank * 8 + kTileThreads - 1) / kTileThreads; ++j)
+                        if (j * 32 + dr < kRank) copy16(stage + d_to + j * 32 * 128, d0 + (int64_t)j * 32 * p.inner + k);
                 }
             }
-            wait_copies<0>();
-            __syncthreads();  // the ring is free for the next round
-            float* v = p.workspace + (part * p.tokens + t0 + warp * 16) * p.rank + r0 + 2 * q;
+            commit_copies();
+        };
+        float acc[kRank / 8][4];
 #pragma unroll
-            for (int n = 0; n < kRank / 8; ++n) {
-                if ((rows >> g) & 1u) *reinterpret_cast<float2*>(v + g * p.rank + n * 8) = make_float2(acc[n][0], acc[n][1]);
-                if ((rows >> (g + 8)) & 1u)
-                    *reinterpret_cast<float2*>(v + (g + 8) * p.rank + n * 8) = make_float2(acc[n][2], acc[n][3]);
+        for (int n = 0; n < kRank / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll
+        for (int s = 0; s < S::kStages - 1; ++s) issue(s);
+        for (int s = 0; s < stages; ++s) {
+            wait_copies<S::kStages - 2>();
+            __syncthreads();  // the stage has arrived for everybody, and the one before has been read by everybody
+            issue(s + S::kStages - 1);
+            if (!busy) continue;
+            const uint8_t* stage = smem + (s % S::kStages) * S::kStage;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                if (s * S::kStepK + i * kStep >= range) break;
+                Fragment<T, 8> a0, a1;
+                load_pieces(a0, stage + (i * kPieces * 2 * kTileThreads + threadIdx.x) * 16, 2 * kTileThreads * 16);
+                load_pieces(a1, stage + ((i * kPieces * 2 + 1) * kTileThreads + threadIdx.x) * 16, 2 * kTileThreads * 16);
+#pragma unroll
+                for (int n0 = 0; n0 < kRank / 8; n0 += kN) {
+                    Fragment<T, 8> b[kN];
+#pragma unroll
+                    for (int n = 0; n < kN; ++n)
+                        load_pieces(b[n], stage + S::kXBytes + ((n0 + n) * 8 + g) * 128 + ((((i * 4 + q) * kPieces) ^ ((g & 1) << 2)) << 4), 16);
+                    multiply<8, kN>(acc + n0, a0, a1, b);
+                }
             }
         }
+        wait_copies<0>();
+        __syncthreads();  // the ring has been read: its memory takes the sums, [128][kRank]
+        float* sums = reinterpret_cast<float*>(smem);
+        float* mine = sums + (warp * 16 + g) * kRank + 2 * q;
+#pragma unroll
+        for (int n = 0; n < kRank / 8; ++n) {
+            *reinterpret_cast<float2*>(mine + n * 8) = make_float2(acc[n][0], acc[n][1]);
+            *reinterpret_cast<float2*>(mine + 8 * kRank + n * 8) = make_float2(acc[n][2], acc[n][3]);
+        }
+        if (parts > 1) cluster.sync(); else __syncthreads();
+        for (int i = part * kTileThreads + threadIdx.x; i < tile.rows * (kRank / 4); i += parts * kTileThreads) {
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c = 0; c < parts; ++c) {
+                const float4 w = reinterpret_cast<const float4*>(parts > 1 ? cluster.map_shared_rank(sums, c) : sums)[i];
+                sum.x += w.x; sum.y += w.y; sum.z += w.z; sum.w += w.w;
+            }
+            *reinterpret_cast<float4*>(p.workspace + (int64_t)(tile.first + i / (kRank / 4)) * p.rank + r0 + i % (kRank / 4) * 4) = sum;
+        }
+        if (parts > 1) cluster.sync(); else __syncthreads();  // the sums have been read
     }
 }
 
 // Expand: the ring passes kExpandCols columns of U_a (rows of the stored matrix) at a time to the CTA's warps, and to every
-// lane the pieces of the base that it will add to.
-constexpr int kExpandCols = 64, kExpandStages = 3;
+// lane the pieces of the base that it will add to.  v, scaled, lies in shared memory as fp32 rows
+// of rank + 4 values (four rows apart: another bank).
+constexpr int kExpandCols = 64;
 template <typename T, typename O, int kRank>
 struct ExpandTile {
     static constexpr int kUBytes = kExpandCols * kRank * (int)sizeof(T);
     static constexpr int kBaseBytes = kTileTokens * kExpandCols * (int)sizeof(O);
     static constexpr int kStage = kUBytes + kBaseBytes;
-    static constexpr int kTotal = kExpandStages * kStage;
+    static constexpr int kStages = sizeof(O) == 4 && kRank == 64 ? 2 : 3;  // (v of rank 256 has to fit beside them)
+    static constexpr int total(int64_t rank) { return kStages * kStage + kTileTokens * ((int)rank + 4) * 4; }
+    static_assert(kStages * kStage + kTileTokens * (256 + 4) * 4 <= 232448 || kRank < 64, "rank 256");
 };
 
 template <typename T, typename O, int kRank>
 __global__ void __launch_bounds__(kTileThreads, 2)
-expand_tile_kernel(AdapterCall p, Units units, int64_t splits) {
+expand_tile_kernel(AdapterCall p, Units units) {
     constexpr int kLen = kRank == 16 ? 4 : 8;
     constexpr int kLoads = kRank / (4 * kLen);
     constexpr int kRowBytes = kRank * (int)sizeof(T);
     constexpr int kRowPieces = kRowBytes / 16;
     constexpr int kSwizzle = kRowPieces >= 8 ? 4 : 0;  // shorter rows: two neighbours share a 128-byte line as they lie
     using S = ExpandTile<T, O, kRank>;
-    constexpr int kStage = S::kStage;
+    constexpr int kStages = S::kStages;
     constexpr int kBaseLen = 16 / (int)sizeof(O), kBasePieces = 8 / kBaseLen;  // of eight consecutive outputs
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int ids[kTileTokens];
-    __shared__ uint32_t words[4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    // the tile's adapters are dealt to `subs` CTAs; those that most tiles have work for come first
-    const int64_t tile = blockIdx.x % units.tiles, part = blockIdx.x / units.tiles % units.parts;
-    const int sub = (int)(blockIdx.x / units.tiles / units.parts);
+    const int64_t part = blockIdx.x / units.tiles;
     const int64_t n0 = part * units.per_part, n1 = min(p.outer, n0 + units.per_part);
-    const int64_t t0 = tile * kTileTokens;
-    const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-
-    TileAdapters adapters = {ids, words};
-    adapters.find(p, t0);
-    if (sub == 0 && p.base != p.out) {  // tokens without an adapter keep their base
-        for (int row = warp; row < kTileTokens; row += kTileWarps) {
-            if (ids[row] != kNone || t0 + row >= p.tokens) continue;
-            for (int64_t n = n0 + lane * 8; n < n1; n += 256) {
-                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                add_base_and_store<O>(p, t0 + row, n, v);
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem);
+    Tile tile;
+    const bool found = tile.find(p, (int)(blockIdx.x % units.tiles));
+    if (!found || tile.id == kNone) {
+        if (found && p.base != p.out) {  // tokens without an adapter keep their base: eight pieces in flight per thread
+            const int per_row = (int)(n1 - n0) / 8, pieces = tile.rows * per_row;
+            for (int i0 = threadIdx.x; i0 < pieces; i0 += 8 * kTileThreads) {
+                Raw8<O> v[8];
+                int64_t at[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = i0 + j * kTileThreads;
+                    at[j] = (tile.first + i / per_row) * p.outer + n0 + i % per_row * 8;
+                    if (i < pieces && p.base != nullptr) v[j].load(static_cast<const O*>(p.base) + at[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    if (p.base != nullptr) v[j].unpack(f);
+                    if (i0 + j * kTileThreads < pieces) store8(static_cast<O*>(p.out) + at[j], f);
+                }
             }
         }
+        wait_for_shrink();
+        return;
     }
+    const int last = tile.first + tile.rows - 1, t0 = tile.first + warp * 16 + g;
+    const bool row0 = t0 <= last, row1 = t0 + 8 <= last, busy = warp * 16 < tile.rows;
     const int chunks = (int)((n1 - n0 + kExpandCols - 1) / kExpandCols);
     const int rounds = (int)(p.rank / kRank);  // a chunk's columns pass in `rounds` pieces of the rank
-    for (int turn = 0;; ++turn) {
-        uint32_t rows;
-        const int id = adapters.next(rows);
-        if (id == kNone) break;
-        if (turn % units.subs != sub) continue;
-        const bool row0 = ((rows >> g) & 1u) != 0, row1 = ((rows >> (g + 8)) & 1u) != 0;
-        const int64_t tok0 = t0 + warp * 16 + g, tok1 = tok0 + 8;
-        const float scale = __ldg(p.scaling + id);
-        const T* up = static_cast<const T*>(p.up) + (int64_t)id * p.outer * p.rank;
-        // what this thread copies into every stage: kUCopies pieces of U, and of the base what it adds to
-        constexpr int kUCopies = (kExpandCols * kRowPieces + kTileThreads - 1) / kTileThreads, kUStep = kTileThreads / kRowPieces;
-        const int ucol = threadIdx.x / kRowPieces, uc = threadIdx.x % kRowPieces;
-        const T* u0 = up + (n0 + ucol) * p.rank + uc * (16 / (int)sizeof(T));
-        const uint32_t u_to = ucol * kRowBytes + ((uc ^ ((ucol & 1) * kSwizzle)) << 4);
-        static_assert(kUStep % 2 == 0, "a thread's columns have one parity");
-        const O* base0 = static_cast<const O*>(p.base) + tok0 * p.outer + n0 + q * 8;
-        const O* base1 = static_cast<const O*>(p.base) + tok1 * p.outer + n0 + q * 8;
-        const bool copy0 = row0 && p.base != nullptr, copy1 = row1 && p.base != nullptr;
-        auto issue = [&](int s) {
-            if (s < chunks * rounds) {
-                const uint32_t stage = base + (s % kExpandStages) * kStage;
-                const int chunk = rounds == 1 ? s : s / rounds, round = rounds == 1 ? 0 : s % rounds;
-                const int n = chunk * kExpandCols, left = (int)(n1 - n0) - n;
-                const T* u = u0 + n * p.rank + round * kRank;
+
+    // what this thread copies into every stage: kUCopies pieces of U, and of the base what it adds to
+    constexpr int kUCopies = (kExpandCols * kRowPieces + kTileThreads - 1) / kTileThreads, kUStep = kTileThreads / kRowPieces;
+    static_assert(kUStep % 2 == 0, "a thread's columns have one parity");
+    const int ucol = threadIdx.x / kRowPieces, uc = threadIdx.x % kRowPieces;
+    const T* u0 = static_cast<const T*>(p.up) + ((int64_t)tile.id * p.outer + n0 + ucol) * p.rank + uc * (16 / (int)sizeof(T));
+    const uint32_t u_to = ucol * kRowBytes + ((uc ^ ((ucol & 1) * kSwizzle)) << 4);
+    const O* base0 = static_cast<const O*>(p.base) + (int64_t)t0 * p.outer + n0 + q * 8;
+    const bool copy0 = row0 && p.base != nullptr, copy1 = row1 && p.base != nullptr;
+    auto issue = [&](int s) {
+        if (s < chunks * rounds) {
+            const uint32_t stage = ring + (s % kStages) * S::kStage;
+            const int chunk = rounds == 1 ? s : s / rounds, round = rounds == 1 ? 0 : s % rounds;
+            const int n = chunk * kExpandCols, left = (int)(n1 - n0) - n;
+            const T* u = u0 + (int64_t)n * p.rank + round * kRank;
 #pragma unroll
-                for (int j = 0; j < kUCopies; ++j)
-                    if (j * kUStep + ucol < kExpandCols && j * kUStep + ucol < left)
-                        copy16(stage + u_to + j * kUStep * kRowBytes, u + (int64_t)j * kUStep * p.rank);
-                if (round == rounds - 1) {
-                    const uint32_t to = stage + S::kUBytes + threadIdx.x * 16;
+            for (int j = 0; j < kUCopies; ++j)
+                if (j * kUStep + ucol < kExpandCols && j * kUStep + ucol < left)
+                    copy16(stage + u_to + j * kUStep * kRowBytes, u + (int64_t)j * kUStep * p.rank);
+            if (round == rounds - 1) {
+                const uint32_t to = stage + S::kUBytes + threadIdx.x * 16;
 #pragma unroll
-                    for (int h = 0; h < kExpandCols / 32; ++h)
-                        if (h * 32 < left) {
+                for (int h = 0; h < kExpandCols / 32; ++h)
+                    if (h * 32 < left) {
 #pragma unroll
-                            for (int e = 0; e < kBasePieces; ++e) {
-                                if (copy0) copy16(to + (h * 2 * kBasePieces + e) * kTileThreads * 16, base0 + n + h * 32 + e * kBaseLen);
-                                if (copy1) copy16(to + ((h * 2 + 1) * kBasePieces + e) * kTileThreads * 16, base1 + n + h * 32 + e * kBaseLen);
-                            }
+                        for (int e = 0; e < kBasePieces; ++e) {
+                            if (copy0) copy16(to + (h * 2 * kBasePieces + e) * kTileThreads * 16, base0 + n + h * 32 + e * kBaseLen);
+                            if (copy1)
+                                copy16(to + ((h * 2 + 1) * kBasePieces + e) * kTileThreads * 16, base0 + 8 * p.outer + n + h * 32 + e * kBaseLen);
                         }
-                }
-            }
-            commit_copies();
-        };
-        SplitFragment<T, kLen> v0[kLoads], v1[kLoads];
-        auto load_rank = [&](int64_t r0) {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int64_t r = r0 + (i * 4 + q) * kLen;
-                load_v<T, kLen>(p, splits, tok0, r, scale, row0, v0[i]);
-                load_v<T, kLen>(p, splits, tok1, r, scale, row1, v1[i]);
-            }
-        };
-#pragma unroll
-        for (int s = 0; s < kExpandStages - 1; ++s) issue(s);
-        if (rounds == 1 && rows != 0) load_rank(0);
-        float acc[kExpandCols / 8][4];
-        for (int s = 0; s < chunks * rounds; ++s) {
-            const int round = s % rounds;
-            const int64_t n = n0 + (int64_t)(s / rounds) * kExpandCols;
-            wait_copies<kExpandStages - 2>();
-            __syncthreads();
-            issue(s + kExpandStages - 1);
-            if (rows == 0) continue;
-            if (rounds > 1) load_rank((int64_t)round * kRank);
-            if (round == 0) {
-#pragma unroll
-                for (int j = 0; j < kExpandCols / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-            }
-            const uint8_t* stage = smem + (s % kExpandStages) * kStage;
-#pragma unroll
-            for (int j0 = 0; j0 < kExpandCols / 8; j0 += kGroup<T>)
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    Fragment<T, kLen> b[kGroup<T>];
-#pragma unroll
-                    for (int j = 0; j < kGroup<T>; ++j) {
-                        const int col = (j0 + j) / 4 * 32 + (g >> 1) * 8 + (j0 + j) % 4 * 2 + (g & 1);
-                        const int c = (i * 4 + q) * kLen * (int)sizeof(T);  // byte in the row
-                        load_pieces(b[j], stage + col * kRowBytes + (c ^ ((g & 1) * kSwizzle * 16)), 16);
                     }
-                    multiply<kLen, kGroup<T>>(acc + j0, v0[i], v1[i], b);
-                }
-            if (round != rounds - 1) continue;
-#pragma unroll
-            for (int h = 0; h < kExpandCols / 32; ++h) {
-                const int64_t c = n + h * 32 + q * 8;
-                if (c >= n1) break;
-                const uint8_t* from = stage + S::kUBytes + (h * 2 * kBasePieces * kTileThreads + threadIdx.x) * 16;
-#pragma unroll
-                for (int second = 0; second < 2; ++second) {
-                    if (second ? !row1 : !row0) continue;
-                    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (p.base != nullptr) {
-                        Raw8<O> b;
-                        b.load_pieces(from + second * kBasePieces * kTileThreads * 16, kTileThreads * 16);
-                        b.unpack(v);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] += acc[h * 4 + (e >> 1)][2 * second + (e & 1)];
-                    store8(static_cast<O*>(p.out) + (second ? tok1 : tok0) * p.outer + c, v);
-                }
             }
         }
-        wait_copies<0>();
-        __syncthreads();  // the ring is free for the next adapter
+        commit_copies();
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) issue(s);
+    const float scale = __ldg(p.scaling + tile.id);
+    wait_for_shrink();
+
+    // v of the tile: rows of rank + 4 floats
+    float* vs = reinterpret_cast<float*>(smem + kStages * S::kStage);
+    const int pitch = (int)p.rank + 4, quads = (int)p.rank / 4;
+    {
+        const float4* src = reinterpret_cast<const float4*>(p.workspace + (int64_t)tile.first * p.rank);
+#pragma unroll 4
+        for (int i = threadIdx.x; i < tile.rows * quads; i += kTileThreads) {
+            float4 sum = src[i];
+            sum.x *= scale; sum.y *= scale; sum.z *= scale; sum.w *= scale;
+            *reinterpret_cast<float4*>(vs + (i / quads) * pitch + (i % quads) * 4) = sum;
+        }
     }
+    __syncthreads();
+    SplitFragment<T, kLen> v0[kLoads], v1[kLoads];
+    auto load_rank = [&](int r0) {  // (rows behind the tile's last read what lies there, and are not stored)
+        const float* v = vs + (warp * 16 + g) * pitch + r0 + q * kLen;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            float a[kLen], b[kLen];
+#pragma unroll
+            for (int e = 0; e < kLen; e += 4) {
+                *reinterpret_cast<float4*>(a + e) = *reinterpret_cast<const float4*>(v + i * 4 * kLen + e);
+                *reinterpret_cast<float4*>(b + e) = *reinterpret_cast<const float4*>(v + 8 * pitch + i * 4 * kLen + e);
+            }
+            v0[i].set(a);
+            v1[i].set(b);
+        }
+    };
+    if (rounds == 1 && busy) load_rank(0);
+    float acc[kExpandCols / 8][4];
+    for (int s = 0; s < chunks * rounds; ++s) {
+        const int chunk = rounds == 1 ? s : s / rounds, round = rounds == 1 ? 0 : s % rounds;
+        wait_copies<kStages - 2>();
+        __syncthreads();
+        issue(s + kStages - 1);
+        if (!busy) continue;
+        if (rounds > 1) load_rank(round * kRank);
+        if (round == 0) {
+#pragma unroll
+            for (int j = 0; j < kExpandCols / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+        }
+        const uint8_t* stage = smem + (s % kStages) * S::kStage;
+#pragma unroll
+        for (int j0 = 0; j0 < kExpandCols / 8; j0 += kGroup<T>)
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                Fragment<T, kLen> b[kGroup<T>];
+#pragma unroll
+                for (int j = 0; j < kGroup<T>; ++j) {
+                    const int col = (j0 + j) / 4 * 32 + (g >> 1) * 8 + (j0 + j) % 4 * 2 + (g & 1);
+                    const int c = (i * 4 + q) * kLen * (int)sizeof(T);  // byte in the row
+                    load_pieces(b[j], stage + col * kRowBytes + (c ^ ((g & 1) * kSwizzle * 16)), 16);
+                }
+                multiply<kLen, kGroup<T>>(acc + j0, v0[i], v1[i], b);
+            }
+        if (round != rounds - 1) continue;
+        const int n = chunk * kExpandCols, left = (int)(n1 - n0) - n;
+        O* out0 = static_cast<O*>(p.out) + (int64_t)t0 * p.outer + n0 + n + q * 8;
+#pragma unroll
+        for (int h = 0; h < kExpandCols / 32; ++h) {
+            if (h * 32 >= left) break;
+            const uint8_t* from = stage + S::kUBytes + (h * 2 * kBasePieces * kTileThreads + threadIdx.x) * 16;
+#pragma unroll
+            for (int second = 0; second < 2; ++second) {
+                if (second ? !row1 : !row0) continue;
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (p.base != nullptr) {
+                    Raw8<O> b;
+                    b.load_pieces(from + second * kBasePieces * kTileThreads * 16, kTileThreads * 16);
+                    b.unpack(v);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += acc[h * 4 + (e >> 1)][2 * second + (e & 1)];
+                store8(out0 + (second ? 8 * p.outer : 0) + h * 32, v);
+            }
+        }
+    }
+    wait_copies<0>();
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -655,31 +701,63 @@ constexpr int64_t kWantedWarps = 148 * 8;
 // Prompts go by tiles of 128 tokens, short requests by warps of 16: TILES_NOTE
 bool by_tiles(int64_t tokens, int64_t requests) { return tokens >= 256 && tokens >= 32 * requests; }
 
-// How the input features are cut: enough warps (or CTAs) to fill the GPU, at least 128 (256) features each, at most 16
-// partial sums.
-Units shrink_units(int64_t tokens, int64_t inner, bool tiles) {
+// How the input features are cut: enough warps to fill the GPU, at least 128 features each, at most 16 partial sums.
+Units shrink_units(int64_t tokens, int64_t inner) {
     Units u;
-    u.tiles = ceil_div(tokens, tiles ? kTileTokens : kTokens);
+    u.tiles = ceil_div(tokens, kTokens);
     u.subs = 1;
-    int64_t parts = tiles ? 148 / u.tiles : ceil_div(kWantedWarps, u.tiles);
+    int64_t parts = ceil_div(kWantedWarps, u.tiles);
     parts = parts < 16 ? parts : 16;
-    const int64_t most = ceil_div(inner, tiles ? 256 : 128);
+    const int64_t most = ceil_div(inner, 128);
     parts = parts < most ? parts : most;
-    parts = parts < 1 ? 1 : parts;
-    u.per_part = ceil_div(ceil_div(inner, parts), 64) * 64;
+    u.per_part = ceil_div(ceil_div(inner, parts), 32) * 32;
     u.parts = ceil_div(inner, u.per_part);
     return u;
 }
 
-// Distinct adapters a warp's 16 tokens may hold: as many as the requests that meet in it, on average.  A tile of 128
-// prompt tokens: 4, because a CTA that serves two adapters takes twice as long as its neighbours, and one without work is
-// gone at once.
-int sub_count(const AdapterCall& p, bool tiles) {
-    if (tiles) return p.requests < 4 ? (int)(p.requests > 1 ? p.requests : 1) : 4;
+// The same for tiles: CTAs of a cluster (a power of two up to 8), two per SM, at least 256 features each.  Tiles start at each
+// request's start, so that there may be one more for every request and for the tokens around them; half that is expected.
+Units tile_units(const AdapterCall& p) {
+    Units u;
+    u.tiles = ceil_div(p.tokens, kTileTokens) + p.requests + 2;
+    u.subs = 1;
+    const int64_t expected = ceil_div(p.tokens, kTileTokens) + p.requests / 2;
+    u.parts = 1;
+    while (u.parts < 8 && expected * u.parts * 2 <= 2 * 148 && u.parts * 2 * 256 <= p.inner) u.parts *= 2;
+    u.per_part = ceil_div(ceil_div(p.inner, u.parts), 64) * 64;
+    return u;
+}
+
+// Distinct adapters a warp's 16 tokens may hold: as many as the requests that meet in it, on average.
+int sub_count(const AdapterCall& p) {
     const int64_t meet = ceil_div(kTokens * p.requests, p.tokens);
     int subs = 1;
     while (subs < meet && subs < kTokens) subs *= 2;
     return subs;
+}
+
+// A launch in clusters of `cluster` CTAs, or one that may begin while the kernel before it still runs.
+template <typename... Params, typename... Args>
+cudaError_t launch_with(void (*kernel)(Params...), int64_t ctas, int threads, int smem, int cluster, bool early,
+                        cudaStream_t stream, Args... args) {
+    if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)ctas);
+    config.blockDim = dim3((unsigned)threads);
+    config.dynamicSmemBytes = (size_t)smem;
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    if (early) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+    } else {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    }
+    config.attrs = attr;
+    config.numAttrs = early || cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
 template <typename Kernel>
@@ -694,35 +772,44 @@ cudaError_t allow_smem(Kernel kernel, int bytes, bool (&ready)[64]) {  // per de
     return err;
 }
 
+// the expand kernel's ranges of output features, in multiples of `unit`, for `wanted` CTAs or warps in all
+void cut_outputs(Units& u, int64_t outer, int64_t unit, int64_t wanted_parts) {
+    const int64_t most = ceil_div(outer, unit);
+    int64_t parts = wanted_parts < most ? wanted_parts : most;
+    parts = parts < 1 ? 1 : parts;
+    u.per_part = ceil_div(most, parts) * unit;
+    u.parts = ceil_div(outer, u.per_part);
+}
+
+template <typename T, typename O, int kRank>
+cudaError_t launch_tiles(const AdapterCall& p, cudaStream_t stream) {
+    const Units shrink = tile_units(p);
+    Units expand = shrink;
+    cut_outputs(expand, p.outer, kExpandCols, 2 * 148 / (ceil_div(p.tokens, kTileTokens) + p.requests / 2));
+    constexpr int kShrinkBytes = ShrinkTile<T, kRank>::kTotal;
+    static bool shrink_ready[64] = {false}, expand_ready[64] = {false};
+    cudaError_t err = allow_smem(shrink_tile_kernel<T, kRank>, kShrinkBytes, shrink_ready);
+    if (err == cudaSuccess)
+        err = allow_smem(expand_tile_kernel<T, O, kRank>, ExpandTile<T, O, kRank>::total(kRank < 64 ? kRank : 256), expand_ready);
+    if (err == cudaSuccess)
+        err = launch_with(shrink_tile_kernel<T, kRank>, shrink.tiles * shrink.parts, kTileThreads, kShrinkBytes, (int)shrink.parts,
+                          false, stream, p, shrink);
+    if (err != cudaSuccess) return err;
+    return launch_with(expand_tile_kernel<T, O, kRank>, expand.tiles * expand.parts, kTileThreads,
+                       ExpandTile<T, O, kRank>::total(p.rank), 1, true, stream, p, expand);
+}
+
 template <typename T, typename O, int kRank>
 cudaError_t launch(const AdapterCall& p, cudaStream_t stream) {
-    const bool tiles = by_tiles(p.tokens, p.requests);
-    Units shrink = shrink_units(p.tokens, p.inner, tiles);
-    Units expand = shrink;
-    shrink.subs = expand.subs = sub_count(p, tiles);
-    const int64_t unit = tiles ? kExpandCols : 32, most = ceil_div(p.outer, unit);
-    int64_t parts = tiles ? 2 * 148 / expand.tiles : ceil_div(kWantedWarps * 2, expand.tiles * expand.subs);
-    parts = parts < most ? parts : most;
-    parts = parts < 1 ? 1 : parts;
-    expand.per_part = ceil_div(most, parts) * unit;
-    expand.parts = ceil_div(p.outer, expand.per_part);
-    const int64_t per_cta = tiles ? 1 : kWarps;
-    const int64_t shrink_ctas = ceil_div(shrink.tiles * shrink.parts * shrink.subs, per_cta);
-    const int64_t expand_ctas = ceil_div(expand.tiles * expand.parts * expand.subs, per_cta);
-    if (shrink_ctas > 0x7fffffffll || expand_ctas > 0x7fffffffll) return cudaErrorInvalidValue;
-    if (tiles) {
-        constexpr int kShrinkBytes = ShrinkTile<T, kRank>::kTotal, kExpandBytes = ExpandTile<T, O, kRank>::kTotal;
-        static bool shrink_ready[64] = {false}, expand_ready[64] = {false};
-        cudaError_t err = allow_smem(shrink_tile_kernel<T, kRank>, kShrinkBytes, shrink_ready);
-        if (err == cudaSuccess) err = allow_smem(expand_tile_kernel<T, O, kRank>, kExpandBytes, expand_ready);
-        if (err != cudaSuccess) return err;
-        shrink_tile_kernel<T, kRank><<<(unsigned)shrink_ctas, kTileThreads, kShrinkBytes, stream>>>(p, shrink);
-        expand_tile_kernel<T, O, kRank><<<(unsigned)expand_ctas, kTileThreads, kExpandBytes, stream>>>(p, expand, shrink.parts);
-    } else {
-        shrink_kernel<T, kRank><<<(unsigned)shrink_ctas, 32 * kWarps, 0, stream>>>(p, shrink);
-        expand_kernel<T, O, kRank><<<(unsigned)expand_ctas, 32 * kWarps, 0, stream>>>(p, expand, shrink.parts);
-    }
-    return cudaGetLastError();
+    if (by_tiles(p.tokens, p.requests)) return launch_tiles<T, O, kRank>(p, stream);
+    Units shrink = shrink_units(p.tokens, p.inner), expand = shrink;
+    shrink.subs = expand.subs = sub_count(p);
+    cut_outputs(expand, p.outer, 32, ceil_div(kWantedWarps * 2, expand.tiles * expand.subs));
+    const cudaError_t err = launch_with(shrink_kernel<T, kRank>, ceil_div(shrink.tiles * shrink.parts * shrink.subs, kWarps),
+                                        32 * kWarps, 0, 1, false, stream, p, shrink);
+    if (err != cudaSuccess) return err;
+    return launch_with(expand_kernel<T, O, kRank>, ceil_div(expand.tiles * expand.parts * expand.subs, kWarps), 32 * kWarps, 0, 1,
+                       true, stream, p, expand, shrink.parts);
 }
 
 template <typename T, typename O>
@@ -737,8 +824,7 @@ cudaError_t by_rank(const AdapterCall& p, cudaStream_t stream) {
 
 int64_t adapters_workspace_bytes(int64_t tokens, int64_t inner, int64_t rank) {
     if (tokens == 0) return 0;
-    const int64_t a = shrink_units(tokens, inner, false).parts, b = shrink_units(tokens, inner, true).parts;
-    return (a > b ? a : b) * tokens * rank * (int64_t)sizeof(float);
+    return shrink_units(tokens, inner).parts * tokens * rank * (int64_t)sizeof(float);  // (tiles: one sum only)
 }
 
 cudaError_t launch_adapters(const AdapterCall& p, bool in_bf16, bool out_bf16, cudaStream_t stream) {
