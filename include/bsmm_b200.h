@@ -323,6 +323,28 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
                      const float* data, int64_t hidden, const float* bias, void* h, uint32_t flags, bsmm_stream_t stream);
 
 /*
+ * The gated block on bf16 tensors with bf16 products (fp32 sums) in one tensor-core kernel: both projections, the activation
+ * and the product.  Where Wg's or Wu's block-row j has a block at an input block, the two form one operand (a missing one as
+ * zeros), so patterns that agree between gate and up cost half of what two separate products would.
+ *   bsmm_build_gated_plan  from the CSR of the 2 * hidden-row matrix; `plan`: bsmm_gated_plan_bytes bytes, 16-byte aligned;
+ *                          depends only on the pattern
+ *   bsmm_gated_pack        bf16 images of the blocks in the plan's order (run it whenever `data` changed); `images`:
+ *                          bsmm_gated_images_bytes bytes, 256-byte aligned
+ *   bsmm_gated_forward     h [m, hidden] bf16; `pre` (bf16 [m, 2 * hidden], may be NULL) receives g and u as bsmm_gated_act's
+ *                          `pre`; flags = BSMM_GATED_IO_BF16 | BSMM_GATED_PRE_BF16, and BSMM_GATED_GELU
+ * k at most BSMM_GATED_MAX_K.  A wait that gives up raises the device health word (bsmm_device_status).
+ */
+#define BSMM_GATED_MAX_K 131072
+int64_t bsmm_gated_plan_bytes(int64_t hidden, int64_t k, int64_t nnz);
+int64_t bsmm_gated_images_bytes(int64_t nnz);
+int bsmm_build_gated_plan(const int32_t* ptr, const int32_t* idx, int64_t hidden, int64_t k, int64_t nnz, void* plan,
+                          bsmm_stream_t stream);
+int bsmm_gated_pack(const float* data, const void* plan, int64_t hidden, int64_t k, int64_t nnz, void* images,
+                    bsmm_stream_t stream);
+int bsmm_gated_forward(const void* x, int64_t m, int64_t k, const void* plan, const void* images, int64_t nnz, int64_t hidden,
+                       const float* bias, void* h, void* pre, uint32_t flags, bsmm_stream_t stream);
+
+/*
  * Dropout with the residual add behind it: out[i] = (keep(i) ? x[i] * 65536 / (65536 - cut) : 0) + residual[i] over n
  * contiguous elements; residual may be NULL.  The mask is never stored: element i draws the (i mod 8)-th 16-bit number (word by
  * word, low half first) of Philox4x32-10 with key rng[0] and 128-bit counter (i / 8, rng[1]) and is kept when the number is

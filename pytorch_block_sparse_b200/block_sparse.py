@@ -515,6 +515,8 @@ class BlockSparseMatrixBase(torch.nn.Module):
         plan = self._plan_cache.get(key)
         if plan is None:
             plan = native.SddmmPlan(ptr, idx)
+            if native.capturing():
+                return plan
             self._plan_cache = {k: v for k, v in self._plan_cache.items() if k[0] != "sddmm"}
             self._plan_cache[key] = plan
         return plan

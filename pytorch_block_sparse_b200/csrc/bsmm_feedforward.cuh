@@ -106,6 +106,16 @@ cudaError_t launch_gated_small(const void* x, int64_t m, int64_t k, const int32_
                                const float* data, int64_t nnz, int64_t hidden, const float* bias, void* h, int act,
                                bool x_bf16, bool h_bf16, cudaStream_t stream);
 
+// the tensor-core forward on bf16 tensors (bsmm_gated_umma.cu)
+int64_t gated_plan_bytes(int64_t hidden, int64_t k, int64_t nnz);
+int64_t gated_images_bytes(int64_t nnz);
+cudaError_t launch_build_gated_plan(const int32_t* ptr, const int32_t* idx, int64_t hidden, int64_t k, void* plan,
+                                    cudaStream_t stream);
+cudaError_t launch_pack_pairs(const float* data, const void* plan, int64_t hidden, int64_t k, int64_t nnz, void* images,
+                              cudaStream_t stream);
+cudaError_t launch_gated_umma(const void* x, int64_t m, int64_t k, const void* plan, const void* images, int64_t hidden,
+                              const float* bias, void* h, void* pre, int act, cudaStream_t stream);
+
 struct AdapterCall {
     const void* x;           // [tokens, inner]
     const void* down;        // [count, rank, inner], rank padded to a multiple of 16 with zero rows

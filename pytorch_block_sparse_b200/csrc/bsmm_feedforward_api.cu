@@ -74,6 +74,46 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
                                                       static_cast<cudaStream_t>(stream)));
 }
 
+int64_t bsmm_gated_plan_bytes(int64_t hidden, int64_t k, int64_t nnz) {
+    if (hidden < 0 || k < 0 || nnz < 0 || (hidden % 32) != 0 || (k % 32) != 0 || nnz > 0x7fffffff || too_large(hidden, k)) return -1;
+    return bsmm::gated_plan_bytes(hidden, k, nnz);
+}
+
+int64_t bsmm_gated_images_bytes(int64_t nnz) { return nnz < 0 || nnz > 0x7fffffff ? -1 : bsmm::gated_images_bytes(nnz); }
+
+int bsmm_build_gated_plan(const int32_t* ptr, const int32_t* idx, int64_t hidden, int64_t k, int64_t nnz, void* plan,
+                          bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (bsmm_gated_plan_bytes(hidden, k, nnz) < 0 || ptr == nullptr || plan == nullptr || (nnz > 0 && idx == nullptr) ||
+        !aligned(ptr, 4) || !aligned(idx, 8) || !aligned(plan, 16))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (k > BSMM_GATED_MAX_K) return BSMM_ERR_TOO_LARGE;
+    return bsmm::report_cuda(bsmm::launch_build_gated_plan(ptr, idx, hidden, k, plan, static_cast<cudaStream_t>(stream)));
+}
+
+int bsmm_gated_pack(const float* data, const void* plan, int64_t hidden, int64_t k, int64_t nnz, void* images,
+                    bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (bsmm_gated_plan_bytes(hidden, k, nnz) < 0 || plan == nullptr || (nnz > 0 && (data == nullptr || images == nullptr)) ||
+        !aligned(data, 16) || !aligned(plan, 16) || !aligned(images, 256))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    return bsmm::report_cuda(bsmm::launch_pack_pairs(data, plan, hidden, k, nnz, images, static_cast<cudaStream_t>(stream)));
+}
+
+int bsmm_gated_forward(const void* x, int64_t m, int64_t k, const void* plan, const void* images, int64_t nnz, int64_t hidden,
+                       const float* bias, void* h, void* pre, uint32_t flags, bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (m < 0 || k <= 0 || nnz < 0 || hidden < 0 || (hidden % 32) != 0 || (k % 32) != 0) return BSMM_ERR_INVALID_ARGUMENT;
+    if ((flags & ~BSMM_GATED_GELU) != (BSMM_GATED_IO_BF16 | BSMM_GATED_PRE_BF16)) return BSMM_ERR_UNSUPPORTED;
+    if (m == 0 || hidden == 0) return BSMM_OK;
+    if (x == nullptr || plan == nullptr || h == nullptr || (nnz > 0 && images == nullptr)) return BSMM_ERR_INVALID_ARGUMENT;
+    if (!aligned(x, 16) || !aligned(plan, 16) || !aligned(images, 256) || !aligned(bias, 16) || !aligned(h, 16) || !aligned(pre, 16))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (nnz > 0x7fffffff || k > BSMM_GATED_MAX_K || too_large(m, k) || too_large(m, 2 * hidden)) return BSMM_ERR_TOO_LARGE;
+    return bsmm::report_cuda(bsmm::launch_gated_umma(x, m, k, plan, images, hidden, bias, h, pre, (flags & BSMM_GATED_GELU) != 0,
+                                                     static_cast<cudaStream_t>(stream)));
+}
+
 int bsmm_dropout(const void* x, const void* residual, void* out, int64_t n, uint32_t cut, const int64_t* rng,
                  uint32_t flags, bsmm_stream_t stream) {
     (void)cudaGetLastError();

@@ -42,9 +42,12 @@ class BlockSparseGatedFunction(torch.autograd.Function):
         # packed once per forward, never cached: writes through ``.data`` do not bump version counters; backward uses the
         # weights that the forward saw
         ctx.packed = weight.packed_weights(precision)
-        out_dtype = _out_dtype(input, precision)
-        pre = weight.reverse_matmul(input.float(), transpose=True, bias=bias, packed=ctx.packed)
-        h = native.gated_act(pre, activation, out_dtype)
+        if _fused(input, precision):
+            # g and u are kept in bf16, the type of every other tensor that this mode keeps for backward
+            h, pre = native.gated_forward(input, _gated_plan(weight), weight_data, bias, activation, True)
+        else:
+            pre = weight.reverse_matmul(input.float(), transpose=True, bias=bias, packed=ctx.packed)
+            h = native.gated_act(pre, activation, _out_dtype(input, precision))
         ctx.save_for_backward(input, pre)
         return h
 
@@ -67,6 +70,25 @@ def _out_dtype(x, precision):
     """bf16 tensors stay bf16 in the 'bf16' precision; every other combination computes fp32 (as BlockSparseLinear)."""
     name = native.default_precision() if precision is None else precision
     return torch.bfloat16 if x.dtype == torch.bfloat16 and name == "bf16" else torch.float32
+
+
+def _fused(x, precision):
+    """Whether the one-kernel forward runs: bf16 tensors in the 'bf16' precision."""
+    return _out_dtype(x, precision) == torch.bfloat16 and x.shape[0] > 0 and x.shape[1] <= native.GATED_MAX_K
+
+
+def _gated_plan(weight):
+    """Cached per-pattern plan of the one-kernel forward, beside the matrix's other plans."""
+    ptr, idx = weight.row_start_ends_a, weight.cols_a
+    key = ("gated", ptr.data_ptr(), ptr._version, idx.data_ptr(), idx._version)
+    plan = weight._plan_cache.get(key)
+    if plan is None:
+        plan = native.GatedPlan(ptr, idx, weight.shape[0] // 2, weight.shape[1])
+        if native.capturing():
+            return plan
+        weight._plan_cache = {k: v for k, v in weight._plan_cache.items() if k[0] != "gated"}
+        weight._plan_cache[key] = plan
+    return plan
 
 
 class BlockSparseGatedLinear(nn.Module):
@@ -173,6 +195,8 @@ class BlockSparseGatedLinear(nn.Module):
         if flat.shape[0] <= SMALL_TOKENS:
             return native.gated_small(flat, weight.row_start_ends_a, weight.cols_a, data, self.hidden_features, bias,
                                       self.activation, out_dtype)
+        if _fused(flat, self.precision):
+            return native.gated_forward(flat, _gated_plan(weight), data, bias, self.activation, False)[0]
         pre = weight.reverse_matmul(flat.float(), transpose=True, bias=bias, precision=self.precision)
         return native.gated_act(pre, self.activation, out_dtype)
 

@@ -54,6 +54,11 @@ EXPORTS = (
     "bsmm_gated_act_workspace_bytes",
     "bsmm_gated_act_backward",
     "bsmm_gated_small",
+    "bsmm_gated_plan_bytes",
+    "bsmm_gated_images_bytes",
+    "bsmm_build_gated_plan",
+    "bsmm_gated_pack",
+    "bsmm_gated_forward",
     "bsmm_dropout",
     "bsmm_rng_next",
     "bsmm_adapters_workspace_bytes",
@@ -139,6 +144,16 @@ def load():
     lib.bsmm_gated_act_backward.argtypes = [vp, vp, i64, i64, vp, vp, vp, u32, vp]
     lib.bsmm_gated_small.restype = i32
     lib.bsmm_gated_small.argtypes = [vp, i64, i64, vp, vp, i64, vp, i64, vp, vp, u32, vp]
+    lib.bsmm_gated_plan_bytes.restype = i64
+    lib.bsmm_gated_plan_bytes.argtypes = [i64, i64, i64]
+    lib.bsmm_gated_images_bytes.restype = i64
+    lib.bsmm_gated_images_bytes.argtypes = [i64]
+    lib.bsmm_build_gated_plan.restype = i32
+    lib.bsmm_build_gated_plan.argtypes = [vp, vp, i64, i64, i64, vp, vp]
+    lib.bsmm_gated_pack.restype = i32
+    lib.bsmm_gated_pack.argtypes = [vp, vp, i64, i64, i64, vp, vp]
+    lib.bsmm_gated_forward.restype = i32
+    lib.bsmm_gated_forward.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, vp, vp, u32, vp]
     lib.bsmm_dropout.restype = i32
     lib.bsmm_dropout.argtypes = [vp, vp, vp, i64, u32, vp, u32, vp]
     lib.bsmm_rng_next.restype = i32
@@ -229,6 +244,12 @@ _HERE = _Here()
 def _on(device):
     """``torch.cuda.device(device)``, which costs a few microseconds, only where another device is current."""
     return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+def capturing():
+    """Whether the current stream is being captured: what is built now is filled by the graph's replays, so it must not be
+    kept for calls outside the graph."""
+    return torch.cuda.is_current_stream_capturing()
 
 
 def _need_cuda(t, name):
@@ -370,7 +391,8 @@ class DsdPlan:
                     ),
                     "bsmm_build_plan",
                 )
-            self._buffers[group] = buf
+            if not capturing():
+                self._buffers[group] = buf
         return buf
 
 
@@ -639,6 +661,59 @@ def gated_small(x, ptr, idx, data, hidden, bias, activation, out_dtype):
             "bsmm_gated_small",
         )
     return out
+
+
+GATED_MAX_K = 131072
+
+
+class GatedPlan:
+    """Launch plan of the gated block's tensor-core kernel for one (offsets, indices) pair of the interleaved matrix."""
+
+    def __init__(self, ptr, idx, hidden, k):
+        _need_cuda(ptr, "ptr")
+        lib = load()
+        self.ptr, self.idx = ptr, idx = _aligned(ptr, 4), _aligned(idx, 8)
+        self.hidden, self.k, self.nnz = hidden, k, idx.shape[0]
+        self.buffer = torch.empty(lib.bsmm_gated_plan_bytes(hidden, k, self.nnz), dtype=torch.uint8, device=ptr.device)
+        with _on(ptr.device):
+            self.stream = _stream(ptr.device)
+            check(lib.bsmm_build_gated_plan(_ptr(ptr), _ptr(idx), hidden, k, self.nnz, _ptr(self.buffer), self.stream),
+                  "bsmm_build_gated_plan")
+            self.event = None if capturing() else torch.cuda.current_stream(ptr.device).record_event()
+
+    def on(self, stream):
+        """The plan's address for work on ``stream``: another stream than the one that built it waits for the build.  (Not
+        while capturing, where an event from outside may not be asked: a capture begins with an idle device.)"""
+        if stream != self.stream and self.event is not None and not capturing():
+            current = torch.cuda.current_stream(self.buffer.device)
+            if not self.event.query():
+                current.wait_event(self.event)
+            self.buffer.record_stream(current)
+        return self.buffer.data_ptr()
+
+
+def gated_forward(x, plan, data, bias, activation, keep_pre):
+    """``(h, pre)`` of the gated block on a contiguous bf16 ``x [m, k]`` (``bsmm_gated_pack`` and ``bsmm_gated_forward``): ``data`` is
+    packed now, ``pre`` is ``None`` unless wanted."""
+    _need_cuda(x, "x")
+    lib = load()
+    m = x.shape[0]
+    x, data, bias = _aligned(x), _aligned(data), _aligned(bias)
+    h = torch.empty((m, plan.hidden), dtype=torch.bfloat16, device=x.device)
+    pre = torch.empty((m, 2 * plan.hidden), dtype=torch.bfloat16, device=x.device) if keep_pre else None
+    images = torch.empty(max(16, lib.bsmm_gated_images_bytes(plan.nnz)), dtype=torch.uint8, device=x.device)
+    flags = _gated_flags(activation) | GATED_IO_BF16 | GATED_PRE_BF16
+    with _on(x.device):
+        stream = _stream(x.device)
+        at = plan.on(stream)
+        check(lib.bsmm_gated_pack(_ptr(data), at, plan.hidden, plan.k, plan.nnz, _ptr(images), stream),
+              "bsmm_gated_pack")
+        check(
+            lib.bsmm_gated_forward(_ptr(x), m, plan.k, at, _ptr(images), plan.nnz, plan.hidden, _ptr(bias),
+                                   _ptr(h), _ptr(pre), flags, stream),
+            "bsmm_gated_forward",
+        )
+    return h, pre
 
 
 def dropout(x, residual, cut, rng):

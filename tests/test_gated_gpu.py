@@ -317,6 +317,61 @@ def test_a_captured_training_step():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("precision", [None, "bf16"])
+def test_a_first_call_under_capture_leaves_nothing_behind(precision):
+    """Plans built while capturing are the graph's: an eager call before any replay must build its own."""
+    layer = make(128, 96, 0.5, precision=precision, seed=11)
+    dtype = torch.bfloat16 if precision else torch.float32
+    x = randn((200, 128), 1).to(dtype).cuda()
+    with torch.no_grad():
+        make(128, 96, 0.5, precision=precision, seed=12)(x)  # the device's first call, with another layer
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layer(x)
+        eager = layer(x)
+        assert rel(eager, reference(layer, x)) <= bound(precision or "tf32x3", 3, dtype)
+        graph.replay()
+        assert torch.equal(out, eager)
+        side = torch.cuda.Stream()
+        layer.weight._plan_cache = {}
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            layer(x)  # builds on the side stream
+        assert torch.equal(layer(x), eager)
+    torch.cuda.synchronize()
+    assert_device_healthy()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("tokens,inner,hidden,density,same", [
+    (33, 32, 32, 1.0, True), (128, 64, 128, 1.0, True), (129, 544, 160, 0.5, True), (400, 1056, 1184, 0.15, False),
+    (300, 4096, 96, 0.6, True), (1500, 256, 4000, 0.3, False), (2049, 96, 2080, 0.05, False),
+])
+def test_the_bf16_kernel_alone(act, tokens, inner, hidden, density, same):
+    """Weights that bf16 holds: only the sums and the output round, so the bar is the output's type (half a step)."""
+    hidden = hidden // 32 * 32
+    g = torch.Generator().manual_seed(tokens)
+    mask = torch.rand((hidden // 16, inner // 32), generator=g) < density
+    if same:
+        mask[1::2] = mask[0::2]
+    layer = make(inner, hidden, act=act, precision="bf16", mask=mask, seed=tokens, bf16_values=True)
+    x, dh = randn((tokens, inner), 6).bfloat16(), randn((tokens, hidden), 7).bfloat16()
+    want = reference(layer, x, dh)
+    with torch.no_grad():
+        h = layer(x.cuda())
+    # each sum of K terms in fp32 is within K 2^-23 of the magnitudes, here far below the output's half step: 1.1 of it
+    assert rel(h, want[0]) <= 1.1 * 2.0 ** -8
+    assert torch.isfinite(h).all()
+    xg = x.cuda().requires_grad_()
+    got = layer(xg)
+    assert torch.equal(got, h)
+    got.backward(dh.cuda())
+    assert rel(xg.grad, want[1]) <= bound("bf16", 4, torch.bfloat16, 1)
+    assert rel(layer.weight.data.grad, in_data_layout(layer, want[2])) <= bound("bf16", 4, roundings=1)
+    assert rel(layer.bias.grad, want[3]) <= bound("bf16", 4, roundings=1)
+    assert_device_healthy()
+
+
 def test_from_linears_and_state_dict():
     torch.manual_seed(0)
     gate, up = torch.nn.Linear(96, 64), torch.nn.Linear(96, 64)
