@@ -6,13 +6,18 @@
 // max(45, N / 2) cycles, so the pair costs what one of its blocks would cost alone; layers built with one pattern for both
 // projections have only full pairs.
 //
-// Tile: 128 tokens x kGroup pair-rows, accumulators in tensor memory, two sets, so that one tile is read out while the next is
-// computed.  A tile visits the input blocks for which the group has a pair (the plan lists them); a visit is one stage of a
-// ring in shared memory: the [128 x 32] slab of x (TMA, 64-byte swizzle) and the visit's pair images, which lie behind one
-// another in memory (packed in the plan's order) and come with one bulk copy.  One CTA per SM walks its tiles.
-//   warp 0     loads: plan -> TMA and bulk copies, and the visit's row mask beside them
-//   warp 1     tcgen05.mma, both operands from shared memory: two k-steps of 16 per pair; one commit per visit
-//   warps 2-5  epilogue: tcgen05.ld, + bias, act(g) * u, (g and u for a backward pass,) stores
+// Tile: 256 tokens (two instructions' M) x two pair-rows, accumulators in tensor memory.  A tile visits the input blocks for
+// which the group has a pair (the plan lists them); a visit is one stage of a ring in shared memory: the [256 x 32] slab of x
+// (TMA, 64-byte swizzle) and the visit's pair images, which lie behind one another in memory (packed in the plan's order) and
+// come with one bulk copy.  One CTA per SM walks its tiles in two pipelines, each with its own half of the ring, of tensor
+// memory and of the warps, a tile at a time each: while one reads its tile out the other computes.
+// What bounds it is the round trip of a stage -- load (~1000 cycles), MMA, commit to the loading warp (~350) -- over the
+// stages that fit: work per visit counts.  (A tile of 128 tokens x four pair-rows, the same memory: 224 us instead of 166 on a
+// prompt of 4001 tokens, 4096 -> 8192 at density 0.25; one pipeline with all of the ring: 227 us.  Without any load, store or
+// read-out the same walk takes 126 us, its MMAs alone 90 us.)
+//   warps 0-3    loads, two per pipeline: plan -> TMA and bulk copies
+//   warps 4-5    tcgen05.mma, both operands from shared memory: two k-steps of 16 per pair; one commit per visit
+//   warps 6-21   epilogue, eight per pipeline: tcgen05.ld, + bias, act(g) * u, (g and u for a backward pass,) stores
 // Every wait is bounded; on expiry the CTA raises the device status word and drains.
 #include <cuda_bf16.h>
 
@@ -25,22 +30,29 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kTileTokens = 128;
-constexpr int kGroup = 4;                    // pair-rows of a tile
-constexpr int kPairCols = 64;                // tensor-memory columns of a pair-row: g | u
-constexpr uint32_t kSlabBytes = kTileTokens * 64;   // [128 tokens][32 k] bf16
+constexpr int kHalves = 2;                   // a tile's tokens, 128 at a time (the M of an instruction)
+constexpr int kTileTokens = 128 * kHalves;
+constexpr int kGroup = 2;                    // pair-rows of a tile
+constexpr int kPairCols = 64;                // tensor-memory columns of a pair-row and half: g | u
+constexpr uint32_t kHalfSlabBytes = 128 * 64;
+constexpr uint32_t kSlabBytes = kTileTokens * 64;   // [256 tokens][32 k] bf16
 constexpr uint32_t kPairBytes = 4096;        // bf16 image of a pair: [64 rows g | u][32 k]
 constexpr uint32_t kStageBytes = kSlabBytes + kGroup * kPairBytes;
-constexpr int kStages = 9;
-constexpr int kBuffers = 2;                  // sets of accumulators
+constexpr int kPipelines = 2;
+constexpr int kStages = 4;                   // of a pipeline
+constexpr int kLoaders = 2;                  // loading warps of a pipeline; a stage stays with one of them
+static_assert(kStages % kLoaders == 0, "a stage stays with one loading warp");
 constexpr uint32_t kTmemCols = 512;
-static_assert(kBuffers * kGroup * kPairCols <= (int)kTmemCols, "tensor memory");
-constexpr uint32_t kOffBar = kStages * kStageBytes;
-constexpr uint32_t kOffCmd = kOffBar + (2 * kStages + 2 * kBuffers) * 8;
-constexpr uint32_t kOffMisc = kOffCmd + kStages * 4;
+constexpr int kAccCols = kHalves * kGroup * kPairCols;  // of a pipeline: [half][row][g | u]
+static_assert(kPipelines * kAccCols <= (int)kTmemCols, "tensor memory");
+constexpr int kBars = 2 * kStages + 2;       // of a pipeline
+constexpr uint32_t kOffBar = kPipelines * kStages * kStageBytes;
+constexpr uint32_t kOffMisc = kOffBar + kPipelines * kBars * 8;
 constexpr uint32_t kSmemBytes = kOffMisc + 16 + 1024;  // + slack to align the base to 1 KiB
 static_assert(kSmemBytes <= 232448, "shared memory");
-constexpr int kThreads = 192;
+constexpr int kFirstMmaWarp = kPipelines * kLoaders, kFirstEpilogueWarp = kFirstMmaWarp + kPipelines;
+constexpr int kEpilogueWarps = 4 * kHalves;  // of a pipeline: every half has its four
+constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps * kPipelines);
 
 // image of a pair: K-major, un-swizzled canonical layout; 8-k chunks of 64 rows x 16 bytes
 constexpr uint32_t kPairLbo = 1024, kPairSbo = 128, kPairStepBytes = 2048;
@@ -58,6 +70,35 @@ struct __align__(16) PlanVisit {
     int32_t rows;        // bit r: row r of the group has a pair here
     int32_t count;       // pairs of the visit
 };
+
+// The MMAs of a visit.  One case per row mask: within it every operand is a constant step from the visit's first, and the
+// single jump costs what one of several conditional branches would.
+template <uint32_t kRows>
+__device__ __forceinline__ void issue_rows(uint32_t acc, uint64_t a, uint64_t w, uint32_t started, int halves) {
+    constexpr uint32_t idesc = make_idesc(1u, 128u, 64u, false, false);
+#pragma unroll
+    for (int half = 0; half < kHalves; ++half) {
+        if (half == 1 && halves == 1) break;
+        const uint64_t tokens = a + (uint64_t)(half * (int)(kHalfSlabBytes >> 4));
+        int at = 0;
+#pragma unroll
+        for (int r = 0; r < kGroup; ++r)
+            if ((kRows >> r) & 1u) {
+                const uint32_t d = acc + (uint32_t)((half * kGroup + r) * kPairCols);
+                const uint64_t image = w + (uint64_t)(at * (int)(kPairBytes >> 4));
+                mma_ss_f16(d, tokens, image, idesc, (started >> r) & 1u);
+                mma_ss_f16(d, tokens + 2, image + (kPairStepBytes >> 4), idesc, 1u);
+                ++at;
+            }
+    }
+}
+__device__ __forceinline__ void issue_visit(uint32_t rows, uint32_t acc, uint64_t a, uint64_t w, uint32_t started, int halves) {
+    switch (rows) {
+        case 1: issue_rows<1>(acc, a, w, started, halves); break;
+        case 2: issue_rows<2>(acc, a, w, started, halves); break;
+        default: issue_rows<3>(acc, a, w, started, halves); break;
+    }
+}
 
 struct GatedParams {
     const PlanGroup* groups;
@@ -85,21 +126,26 @@ gated_umma_kernel(const __grid_constant__ CUtensorMap tmap_x, const GatedParams 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-    auto full = [&](int s) { return smem_base + kOffBar + 8u * s; };
-    auto empty = [&](int s) { return smem_base + kOffBar + 8u * (kStages + s); };
-    auto acc_full = [&](int b) { return smem_base + kOffBar + 8u * (2 * kStages + b); };
-    auto acc_empty = [&](int b) { return smem_base + kOffBar + 8u * (2 * kStages + kBuffers + b); };
-    auto cmd = [&](int s) { return smem_base + kOffCmd + 4u * s; };
-    volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem_gen + kOffMisc);  // [0] tensor memory, [1] abort
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int pl = warp < kFirstMmaWarp ? warp / kLoaders
+                   : warp < kFirstEpilogueWarp ? warp - kFirstMmaWarp : (warp - kFirstEpilogueWarp) / kEpilogueWarps;  // pipeline
+    const uint32_t bars = smem_base + kOffBar + (uint32_t)(pl * kBars) * 8u;
+    const uint32_t ring = smem_base + (uint32_t)(pl * kStages) * kStageBytes;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (kStages + s); };
+    const uint32_t acc_full = bars + 8u * (2 * kStages), acc_empty = acc_full + 8u;
+    volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem_gen + kOffMisc);  // [0] tensor memory, [1] abort
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int b = 0; b < kBuffers; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 128); }
+        for (int q = 0; q < kPipelines; ++q) {
+            const uint32_t at = smem_base + kOffBar + (uint32_t)(q * kBars) * 8u;
+            for (int i = 0; i <= 2 * kStages; ++i) mbar_init(at + 8u * i, 1);
+            mbar_init(at + 8u * (2 * kStages + 1), 32 * kEpilogueWarps);
+        }
         misc[1] = 0;
         fence_mbar_init();
     }
-    if (warp == 1) {
+    if (warp == kFirstMmaWarp) {
         tmem_alloc(smem_base + kOffMisc, kTmemCols);
         tmem_relinquish();
     }
@@ -114,101 +160,125 @@ gated_umma_kernel(const __grid_constant__ CUtensorMap tmap_x, const GatedParams 
         if (!__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag))) bad = true;
     };
 
-    if (warp == 0) {
+    const int tile0 = (int)blockIdx.x + pl * (int)gridDim.x, tile_step = kPipelines * (int)gridDim.x;
+    if (warp < kFirstMmaWarp) {
         // ------------------------------------------------------------------ loads
-        uint32_t seq = 0;  // visits so far, over all tiles
-        for (int tile = blockIdx.x; tile < p.n_tiles && !bad; tile += gridDim.x) {
+        const int part = warp % kLoaders;
+        int done = 0;              // visits of earlier tiles
+        int s = part;              // stage of this warp's next visit, and the parity of its release
+        uint32_t parity = 1;
+        uint32_t issued = 0;
+        for (int tile = tile0; tile < p.n_tiles && !bad; tile += tile_step) {
             const int g = tile % p.n_groups;
             const int32_t tok0 = tile / p.n_groups * kTileTokens;
             const int visits = __ldg(&p.groups[g].visits);
             const int4* list = reinterpret_cast<const int4*>(p.visits + (int64_t)g * p.k_blocks);
-            int4 ahead = lane < visits ? __ldg(list + lane) : make_int4(0, 0, 0, 0);
-            for (int base = 0; base < visits && !bad; base += 32) {
+            // this warp's visits: those whose number over all tiles is `part` mod kLoaders; lane i holds the i-th of a chunk
+            const int begin = (part + kLoaders - done % kLoaders) % kLoaders;
+            auto fetch = [&](int i) { return i < visits ? __ldg(list + i) : make_int4(0, 0, 0, 0); };
+            int4 ahead = fetch(begin + lane * kLoaders);
+            for (int base = begin; base < visits && !bad; base += 32 * kLoaders) {
                 const int4 mine = ahead;
-                ahead = base + 32 + lane < visits ? __ldg(list + base + 32 + lane) : make_int4(0, 0, 0, 0);
-                const int n = min(32, visits - base);
-                for (int i = 0; i < n; ++i, ++seq) {
-                    const int s = (int)(seq % kStages);
+                ahead = fetch(base + (32 + lane) * kLoaders);
+                const int n = min(32, (visits - base + kLoaders - 1) / kLoaders);
+                for (int i = 0; i < n; ++i) {
                     const int inner = __shfl_sync(0xffffffffu, mine.x, i), pair = __shfl_sync(0xffffffffu, mine.y, i);
-                    const int rows = __shfl_sync(0xffffffffu, mine.z, i), count = __shfl_sync(0xffffffffu, mine.w, i);
-                    wait(empty(s), ((seq / kStages) & 1u) ^ 1u);
-                    const uint32_t stage = smem_base + s * kStageBytes;
+                    const int count = __shfl_sync(0xffffffffu, mine.w, i);
+                    wait(empty(s), parity);
+                    const uint32_t stage = ring + s * kStageBytes;
                     if (elect_one() && !bad) {
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(cmd(s)), "r"(rows) : "memory");
                         mbar_arrive_expect_tx(full(s), p.x_bytes + (uint32_t)count * kPairBytes);
                         tma_load_2d(stage, &tmap_x, inner * 32, tok0, full(s));
                         bulk_load(stage + kSlabBytes, p.images + (int64_t)pair * kPairBytes, (uint32_t)count * kPairBytes, full(s));
                     }
+                    if (!bad) ++issued;
+                    s += kLoaders;
+                    if (s >= kStages) { s -= kStages; parity ^= 1u; }
                 }
             }
+            done += visits;
         }
         if (bad) {  // the copies still in flight land in this CTA's memory: they are waited for, again with a limit
-            for (uint32_t v = seq > kStages ? seq - kStages : 0; v < seq; ++v) {
+            constexpr uint32_t kMine = kStages / kLoaders;
+            for (uint32_t v = issued > kMine ? issued - kMine : 0; v < issued; ++v) {
                 const long long t0 = clock64();
-                while (!mbar_test_wait(full((int)(v % kStages)), (v / kStages) & 1u) && clock64() - t0 < kWaitCycles / 16) {}
+                while (!mbar_test_wait(full((int)(v % kMine) * kLoaders + part), (v / kMine) & 1u) && clock64() - t0 < kWaitCycles / 16) {}
             }
         }
-    } else if (warp == 1) {
+    } else if (warp < kFirstEpilogueWarp) {
         // ------------------------------------------------------------------ MMA
-        constexpr uint32_t idesc = make_idesc(1u, 128u, 64u, false, false);
-        uint32_t seq = 0, turn = 0;
-        for (int tile = blockIdx.x; tile < p.n_tiles && !bad; tile += gridDim.x, ++turn) {
-            const int g = tile % p.n_groups, b = (int)(turn % kBuffers);
-            const int visits = __ldg(&p.groups[g].visits);
-            const uint32_t acc = tmem + (uint32_t)(b * kGroup * kPairCols);
-            wait(acc_empty(b), ((turn / kBuffers) & 1u) ^ 1u);
+        const uint64_t a0 = smem_desc_sw64(ring, 16u, 512u);
+        const uint64_t w0 = smem_desc_noswizzle(ring + kSlabBytes, kPairLbo, kPairSbo);
+        const uint32_t acc = tmem + (uint32_t)(pl * kAccCols);
+        int s = 0;
+        uint32_t parity = 0, acc_parity = 1;
+        for (int tile = tile0; tile < p.n_tiles && !bad; tile += tile_step) {
+            const int visits = __ldg(&p.groups[tile % p.n_groups].visits);
+            const int halves = (int64_t)(tile / p.n_groups) * kTileTokens + 128 < p.m ? 2 : 1;  // the second one may lie behind the tokens
+            wait(acc_empty, acc_parity);
+            acc_parity ^= 1u;
             tc_fence_after();
-            uint32_t started = 0;
-            for (int i = 0; i < visits && !bad; ++i, ++seq) {
-                const int s = (int)(seq % kStages);
-                wait(full(s), (seq / kStages) & 1u);
-                uint32_t rows;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(rows) : "r"(cmd(s)) : "memory");
-                const uint32_t stage = smem_base + s * kStageBytes;
-                const uint64_t a = smem_desc_sw64(stage, 16u, 512u);
-                uint64_t w = smem_desc_noswizzle(stage + kSlabBytes, kPairLbo, kPairSbo);
-                if (elect_one() && !bad) {
-#pragma unroll
-                    for (int r = 0; r < kGroup; ++r)
-                        if ((rows >> r) & 1u) {
-                            mma_ss_f16(acc + r * kPairCols, a, w, idesc, (started >> r) & 1u);
-                            mma_ss_f16(acc + r * kPairCols, a + 2, w + (kPairStepBytes >> 4), idesc, 1u);
-                            w += kPairBytes >> 4;
-                        }
-                    mma_commit(empty(s));
+            // lane i holds the row mask of visit base + i; a visit's mask is made warp-uniform (a reduction) one visit ahead, and
+            // the next stage's barrier is tested before the current visit is issued, so that both answers arrive on the way
+            const int4* list = reinterpret_cast<const int4*>(p.visits + (int64_t)(tile % p.n_groups) * p.k_blocks);
+            auto fetch = [&](int i) { return i < visits ? (uint32_t)__ldg(&list[i].z) : 0u; };
+            uint32_t masks = fetch(lane), ahead = fetch(32 + lane);
+            uint32_t started = 0;  // bit r: row r holds a sum of this tile
+            uint32_t rows = __reduce_or_sync(0xffffffffu, lane == 0 ? masks : 0u);
+            bool arrived = mbar_test_wait(full(s), parity);
+            for (int i = 0; i < visits; ++i) {
+                if (!__all_sync(0xffffffffu, arrived)) {
+                    wait(full(s), parity);
+                    if (bad) break;
+                }
+                const int now = s;
+                if (++s == kStages) { s = 0; parity ^= 1u; }
+                arrived = mbar_test_wait(full(s), parity);
+                const int next = (i + 1) & 31;
+                if (next == 0) {
+                    masks = ahead;
+                    ahead = fetch(i + 33 + lane);
+                }
+                const uint32_t rows_next = __reduce_or_sync(0xffffffffu, lane == next ? masks : 0u);
+                const uint64_t a = a0 + (uint64_t)(now * (int)(kStageBytes >> 4)), w = w0 + (uint64_t)(now * (int)(kStageBytes >> 4));
+                if (elect_one()) {
+                    issue_visit(rows, acc, a, w, started, halves);
+                    mma_commit(empty(now));
                 }
                 started |= rows;
+                rows = rows_next;
             }
-            if (elect_one() && !bad) mma_commit(acc_full(b));
+            if (elect_one() && !bad) mma_commit(acc_full);
         }
     } else {
         // ------------------------------------------------------------------ epilogue
-        const int quarter = warp & 3;
-        const uint32_t tmem_lane = tmem + ((uint32_t)(quarter * 32) << 16);
-        uint32_t turn = 0;
-        for (int tile = blockIdx.x; tile < p.n_tiles; tile += gridDim.x, ++turn) {
-            const int g = tile % p.n_groups, b = (int)(turn % kBuffers);
-            const int64_t tok = (int64_t)(tile / p.n_groups) * kTileTokens + quarter * 32 + lane;
+        const int quarter = warp & 3, half = (warp - kFirstEpilogueWarp) / 4 % kHalves;
+        const uint32_t tmem_lane = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(pl * kAccCols + half * kGroup * kPairCols);
+        uint32_t parity = 0;
+        for (int tile = tile0; tile < p.n_tiles; tile += tile_step) {
+            const int g = tile % p.n_groups;
+            const int64_t tok = (int64_t)(tile / p.n_groups) * kTileTokens + half * 128 + quarter * 32 + lane;
             const uint32_t rows = (uint32_t)__ldg(&p.groups[g].rows);
-            wait(acc_full(b), (turn / kBuffers) & 1u);
+            wait(acc_full, parity);
+            parity ^= 1u;
             if (bad) break;
             tc_fence_after();
-            for (int r = 0; r < kGroup; ++r) {
-                const int row = g * kGroup + r;
-                if (row >= p.n_rows) break;
-                uint32_t gate[32], up[32];
+            for (int part = 0; part < 2 * kGroup; ++part) {  // 16 hidden units of a row
+                const int r = part >> 1, c = (part & 1) * 16, row = g * kGroup + r;
+                if (row >= p.n_rows || tok - lane >= p.m) continue;
+                uint32_t gate[16], up[16];
                 if ((rows >> r) & 1u) {
-                    tmem_ld32(tmem_lane + (uint32_t)((b * kGroup + r) * kPairCols), gate);
-                    tmem_ld32(tmem_lane + (uint32_t)((b * kGroup + r) * kPairCols + 32), up);
+                    tmem_ld16(tmem_lane + (uint32_t)(r * kPairCols + c), gate);
+                    tmem_ld16(tmem_lane + (uint32_t)(r * kPairCols + 32 + c), up);
                     tmem_wait_ld();
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) gate[j] = up[j] = 0;
+                    for (int j = 0; j < 16; ++j) gate[j] = up[j] = 0;
                 }
                 if (p.bias != nullptr) {
-                    const float4* bias = reinterpret_cast<const float4*>(p.bias + (int64_t)row * 64);
+                    const float4* bias = reinterpret_cast<const float4*>(p.bias + (int64_t)row * 64 + c);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < 4; ++j) {
                         const float4 bg = __ldg(bias + j), bu = __ldg(bias + 8 + j);
                         gate[4 * j] = __float_as_uint(__uint_as_float(gate[4 * j]) + bg.x);
                         gate[4 * j + 1] = __float_as_uint(__uint_as_float(gate[4 * j + 1]) + bg.y);
@@ -221,9 +291,9 @@ gated_umma_kernel(const __grid_constant__ CUtensorMap tmap_x, const GatedParams 
                     }
                 }
                 if (p.pre != nullptr && tok < p.m) {
-                    __nv_bfloat16* pre = p.pre + tok * 2 * p.hidden + (int64_t)row * 64;
+                    __nv_bfloat16* pre = p.pre + tok * 2 * p.hidden + (int64_t)row * 64 + c;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < 2; ++j) {
                         float v[8], w[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) { v[e] = __uint_as_float(gate[8 * j + e]); w[e] = __uint_as_float(up[8 * j + e]); }
@@ -231,10 +301,10 @@ gated_umma_kernel(const __grid_constant__ CUtensorMap tmap_x, const GatedParams 
                         store8(pre + 32 + 8 * j, w);
                     }
                 }
-                __nv_bfloat16* h = p.h + tok * p.hidden + (int64_t)row * 32;
+                __nv_bfloat16* h = p.h + tok * p.hidden + (int64_t)row * 32 + c;
                 auto finish = [&](int kind) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < 2; ++j) {
                         float v[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
@@ -245,14 +315,14 @@ gated_umma_kernel(const __grid_constant__ CUtensorMap tmap_x, const GatedParams 
                 if (p.act == 0) finish(0); else finish(1);
             }
             tc_fence_before();
-            mbar_arrive(acc_empty(b));
+            mbar_arrive(acc_empty);
         }
     }
 
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag != 0) atomicOr(p.status, 1u);
-    if (warp == 1) {
+    if (warp == kFirstMmaWarp) {
         __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
@@ -325,30 +395,47 @@ build_gated_plan_kernel(const int32_t* __restrict__ ptr, const int2* __restrict_
 }
 
 // ---------------------------------------------------------------------------------------------------------------- pack
-// The bf16 image of every pair, [gate rows | up rows] x k, from the two blocks' T[c][r] = W[r][c].  Memory bound.
+// The bf16 image of every pair, [gate rows | up rows] x k, from the two blocks' T[c][r] = W[r][c].  Memory bound; a CTA takes
+// kPackPairs pairs and asks for all of their blocks at once (one pair per CTA: 23 us for 67 MB of blocks, four: the same; what is left is the
+// ramp of a short kernel: the floor is 15 us).
+constexpr int kPackPairs = 4;
 __global__ void __launch_bounds__(256)
-pack_pairs_kernel(const float* __restrict__ data, const int2* __restrict__ pairs, uint8_t* __restrict__ images) {
-    __shared__ float T[2][32][33];
-    const int2 slots = pairs[blockIdx.x];
-    if (slots.x < 0 && slots.y < 0) return;  // fewer pairs than entries
+pack_pairs_kernel(const float* __restrict__ data, const int2* __restrict__ pairs, int64_t count, uint8_t* __restrict__ images) {
+    __shared__ float T[kPackPairs][2][32][33];
     const int tid = threadIdx.x, c = tid >> 3, r4 = (tid & 7) * 4;
+    const int64_t first = (int64_t)blockIdx.x * kPackPairs;
+    int2 slots[kPackPairs];
+    float4 v[kPackPairs][2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int slot = half == 0 ? slots.x : slots.y;
-        const float4 v = slot < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+    for (int i = 0; i < kPackPairs; ++i) slots[i] = first + i < count ? __ldg(pairs + first + i) : make_int2(-1, -1);
+#pragma unroll
+    for (int i = 0; i < kPackPairs; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int slot = half == 0 ? slots[i].x : slots[i].y;
+            v[i][half] = slot < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
                                   : __ldg(reinterpret_cast<const float4*>(data + (int64_t)slot * kBlockElems) + tid);
-        T[half][c][r4 + 0] = v.x;
-        T[half][c][r4 + 1] = v.y;
-        T[half][c][r4 + 2] = v.z;
-        T[half][c][r4 + 3] = v.w;
-    }
-    __syncthreads();
-    // 16 bytes per thread: chunk of 8 k, one of 64 rows
-    const int chunk = tid >> 6, row = tid & 63, half = row >> 5, r = row & 31;
-    float v[8];
+        }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = T[half][chunk * 8 + j][r];
-    store8(reinterpret_cast<__nv_bfloat16*>(images + (int64_t)blockIdx.x * kPairBytes + tid * 16), v);
+    for (int i = 0; i < kPackPairs; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            T[i][half][c][r4 + 0] = v[i][half].x;
+            T[i][half][c][r4 + 1] = v[i][half].y;
+            T[i][half][c][r4 + 2] = v[i][half].z;
+            T[i][half][c][r4 + 3] = v[i][half].w;
+        }
+    __syncthreads();
+    // 16 bytes per thread and pair: chunk of 8 k, one of 64 rows
+    const int chunk = tid >> 6, row = tid & 63, half = row >> 5, r = row & 31;
+#pragma unroll
+    for (int i = 0; i < kPackPairs; ++i) {
+        if (slots[i].x < 0 && slots[i].y < 0) continue;  // fewer pairs than entries
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = T[i][half][chunk * 8 + j][r];
+        store8(reinterpret_cast<__nv_bfloat16*>(images + (first + i) * kPairBytes + tid * 16), w);
+    }
 }
 
 int64_t group_count(int64_t hidden) { return (hidden / 32 + kGroup - 1) / kGroup; }
@@ -387,7 +474,8 @@ cudaError_t launch_pack_pairs(const float* data, const void* plan, int64_t hidde
                               cudaStream_t stream) {
     if (nnz == 0) return cudaSuccess;
     const PlanPointers at = plan_pointers(const_cast<void*>(plan), hidden, k);
-    pack_pairs_kernel<<<(unsigned)nnz, 256, 0, stream>>>(data, at.pairs, static_cast<uint8_t*>(images));
+    pack_pairs_kernel<<<(unsigned)((nnz + kPackPairs - 1) / kPackPairs), 256, 0, stream>>>(data, at.pairs, nnz,
+                                                                                           static_cast<uint8_t*>(images));
     return cudaGetLastError();
 }
 
