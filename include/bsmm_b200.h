@@ -323,6 +323,30 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
                      const float* data, int64_t hidden, const float* bias, void* h, uint32_t flags, bsmm_stream_t stream);
 
 /*
+ * The whole forward and backward pass of the gated block on fp32 tensors (bf16 ones in BSMM_PREC_BF16's backward pass), each
+ * one call that enqueues the calls above and those of the matrix in order: packing, product, activation; activation's gradient,
+ * weight gradient, input gradient.  One call instead of three is what a training step of a small layer is bound by.
+ *   ptr / idx, plan            CSR of the 2 * hidden-row matrix, and bsmm_build_plan of it (FP32_SIMT: NULL)
+ *   csc_ptr / csc_idx, csc_plan  the same of the CSC
+ *   blocks, sddmm_plan         for the weight gradient, as bsmm_sddmm
+ *   packed                     bsmm_packed_bytes bytes: written by the forward pass, read by the backward pass
+ *   flags                      precision, BSMM_DSD_GROUP(g) of `plan` (forward) or `csc_plan` (backward),
+ *                              BSMM_GATED_PASS(activation and type flags as for bsmm_gated_act)
+ *   dx, dw, dbias              NULL where not wanted; block_sumsq as bsmm_sddmm
+ *   workspace                  bsmm_gated_backward_workspace_bytes bytes, 16-byte aligned
+ */
+#define BSMM_GATED_PASS(f) (((uint32_t)(f)&0xFu) << 16)
+int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, int64_t nnz,
+                            const float* data, void* packed, const void* plan, int64_t hidden, const float* bias, float* pre,
+                            void* h, uint32_t flags, bsmm_stream_t stream);
+int64_t bsmm_gated_backward_workspace_bytes(int64_t m, int64_t k, int64_t hidden, int64_t nnz, uint32_t flags);
+int bsmm_gated_pass_backward(const void* x, const void* pre, const void* dh, int64_t m, int64_t k, const int32_t* idx,
+                             const int32_t* csc_ptr, const int32_t* csc_idx, const int32_t* blocks, int64_t nnz,
+                             const float* data, const void* packed, const void* csc_plan, const void* sddmm_plan,
+                             int64_t hidden, void* dpre, void* dx, float* dw, float* dbias, float* block_sumsq,
+                             void* workspace, uint32_t flags, bsmm_stream_t stream);
+
+/*
  * The gated block on bf16 tensors with bf16 products (fp32 sums) in one tensor-core kernel: both projections, the activation
  * and the product.  Where Wg's or Wu's block-row j has a block at an input block, the two form one operand (a missing one as
  * zeros), so patterns that agree between gate and up cost half of what two separate products would.

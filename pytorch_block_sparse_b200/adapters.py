@@ -97,33 +97,39 @@ class LowRankAdapters(nn.Module):
         zeros).  ``x [..., in]`` in the adapters' type, its leading dimensions flattened to the batch's tokens;
         ``base [..., out]`` in the same type or fp32.  ``inplace`` adds into ``base`` (contiguous) and returns it.  ``dtype``: the
         output's type where there is no base, ``x``'s (the default) or fp32."""
-        if torch.is_grad_enabled() and (x.requires_grad or (base is not None and base.requires_grad)):
+        if (x.requires_grad or (base is not None and base.requires_grad)) and torch.is_grad_enabled():
             raise native.NativeError("LowRankAdapters serve and have no gradients: call them under torch.no_grad()")
+        buffers = self._buffers
+        down, up, scaling = buffers["down"], buffers["up"], buffers["scaling"]
+        lead, kind = x.shape[:-1], x.dtype
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise Exception("Invalid input %s for adapters of %d features" % (tuple(x.shape), self.in_features))
-        if x.dtype != self.down.dtype:
-            raise ValueError("x is %s, the adapters are %s" % (x.dtype, self.down.dtype))
-        for name, t in (("x", x), ("offsets", requests.offsets), ("base", base)):
-            if t is not None and t.device != self.down.device:
-                raise native.NativeError("%s is on %s, the adapters are on %s" % (name, t.device, self.down.device))
-        shape = tuple(x.shape[:-1]) + (self.out_features,)
+        if kind is not down.dtype:
+            raise ValueError("x is %s, the adapters are %s" % (kind, down.dtype))
+        device = down.device
+        if x.device != device or requests.offsets.device != device or (base is not None and base.device != device):
+            raise native.NativeError("x, the requests, the base and the adapters must be on one device, got %s, %s, %s, %s" % (
+                x.device, requests.offsets.device, base.device if base is not None else None, device))
         if base is not None:
-            if tuple(base.shape) != shape:
-                raise ValueError("base must be %s, got %s" % (shape, tuple(base.shape)))
-            if base.dtype not in (x.dtype, torch.float32):
-                raise ValueError("base is %s: expected %s or float32" % (base.dtype, x.dtype))
+            if base.shape != lead + (self.out_features,):
+                raise ValueError("base must be %s, got %s" % (tuple(lead) + (self.out_features,), tuple(base.shape)))
+            kind = base.dtype
+        elif dtype is not None:
+            kind = dtype
+        if kind is not x.dtype and kind is not torch.float32:
+            raise ValueError("the output's type is %s: expected %s or float32" % (kind, x.dtype))
         if inplace:
             if base is None or not base.is_contiguous() or base.data_ptr() % 16 != 0:
                 raise ValueError("inplace wants a contiguous, 16-byte aligned base")
             out = base
         else:
-            kind = base.dtype if base is not None else x.dtype if dtype is None else dtype
-            if kind not in (x.dtype, torch.float32):
-                raise ValueError("dtype is %s: expected %s or float32" % (kind, x.dtype))
-            out = torch.empty(shape, dtype=kind, device=x.device)
-            base = native._aligned(base.contiguous()) if base is not None else None
-        native.adapters(x.reshape(-1, self.in_features).contiguous(), requests.offsets, requests.adapters,
-                        native._aligned(self.down), native._aligned(self.up), self.scaling, base, out)
+            out = torch.empty(lead + (self.out_features,), dtype=kind, device=device)
+            if base is not None:
+                base = native._aligned(base.contiguous())
+        if x.dim() != 2:
+            x = x.reshape(-1, self.in_features)
+        native.adapters(x.contiguous(), requests.offsets, requests.adapters, native._aligned(down), native._aligned(up), scaling,
+                        base, out)
         return out
 
     def extra_repr(self):

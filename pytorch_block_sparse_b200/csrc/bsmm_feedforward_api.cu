@@ -74,6 +74,49 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
                                                       static_cast<cudaStream_t>(stream)));
 }
 
+int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, int64_t nnz,
+                            const float* data, void* packed, const void* plan, int64_t hidden, const float* bias, float* pre,
+                            void* h, uint32_t flags, bsmm_stream_t stream) {
+    const uint32_t precision = flags & BSMM_PREC_MASK, pass = (flags >> 16) & 0xFu;
+    if ((flags & ~(BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF) | BSMM_GATED_PASS(0xF))) != 0 || (pass & BSMM_GATED_PRE_BF16) != 0)
+        return BSMM_ERR_UNSUPPORTED;
+    if (precision != BSMM_PREC_FP32_SIMT) {
+        const int status = bsmm_pack_weights(data, nnz, precision, packed, nullptr, stream);
+        if (status != BSMM_OK) return status;
+    }
+    const int status = bsmm_dsd(x, m, k, ptr, idx, nnz, data, packed, plan, 2 * hidden, pre, bias,
+                                flags & (BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF)), stream);
+    return status != BSMM_OK ? status : bsmm_gated_act(pre, m, hidden, h, pass, stream);
+}
+
+// the bias gradient's partial sums and the weight gradient's: one after the other, in the same memory
+int64_t bsmm_gated_backward_workspace_bytes(int64_t m, int64_t k, int64_t hidden, int64_t nnz, uint32_t flags) {
+    const int64_t a = bsmm_gated_act_workspace_bytes(m, hidden);
+    const int64_t b = bsmm_sddmm_workspace_bytes(2 * hidden, k, m, nnz, flags & BSMM_PREC_MASK);
+    return a < 0 || b < 0 ? -1 : a > b ? a : b;
+}
+
+int bsmm_gated_pass_backward(const void* x, const void* pre, const void* dh, int64_t m, int64_t k, const int32_t* idx,
+                             const int32_t* csc_ptr, const int32_t* csc_idx, const int32_t* blocks, int64_t nnz,
+                             const float* data, const void* packed, const void* csc_plan, const void* sddmm_plan,
+                             int64_t hidden, void* dpre, void* dx, float* dw, float* dbias, float* block_sumsq,
+                             void* workspace, uint32_t flags, bsmm_stream_t stream) {
+    const uint32_t precision = flags & BSMM_PREC_MASK, pass = (flags >> 16) & 0xFu;
+    if ((flags & ~(BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF) | BSMM_GATED_PASS(0xF))) != 0) return BSMM_ERR_UNSUPPORTED;
+    // bf16 tensors: the products take them as they are, which the CUDA-core kernels of few tokens or no blocks do not
+    const bool io16 = (pass & BSMM_GATED_IO_BF16) != 0;
+    if (io16 && (precision != BSMM_PREC_BF16 || m < 32 || nnz == 0)) return BSMM_ERR_UNSUPPORTED;
+    int status = bsmm_gated_act_backward(pre, dh, m, hidden, dpre, dbias, workspace, pass, stream);
+    // the weight gradient first: in data-parallel training its all-reduce can overlap the input gradient
+    if (status == BSMM_OK && dw != nullptr)
+        status = bsmm_sddmm(dpre, x, 2 * hidden, k, m, dw, blocks, nnz, idx, sddmm_plan, block_sumsq, workspace,
+                            precision | (io16 ? BSMM_SDDMM_IO_BF16 : 0u), stream);
+    if (status == BSMM_OK && dx != nullptr)
+        status = bsmm_dsd(dpre, m, 2 * hidden, csc_ptr, csc_idx, nnz, data, packed, csc_plan, k, dx, nullptr,
+                          (flags & (BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF))) | BSMM_DSD_DGRAD | (io16 ? BSMM_DSD_IO_BF16 : 0u), stream);
+    return status;
+}
+
 int64_t bsmm_gated_plan_bytes(int64_t hidden, int64_t k, int64_t nnz) {
     if (hidden < 0 || k < 0 || nnz < 0 || (hidden % 32) != 0 || (k % 32) != 0 || nnz > 0x7fffffff || too_large(hidden, k)) return -1;
     return bsmm::gated_plan_bytes(hidden, k, nnz);

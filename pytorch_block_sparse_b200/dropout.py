@@ -5,7 +5,6 @@ The reference leaves both to the model (a ``torch.nn.Dropout`` and an addition a
 output projection of a block-sparse layer (``BlockSparseLinear(dropout=p)``) and by themselves.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import native
 
@@ -35,11 +34,15 @@ class DropoutResidualFunction(torch.autograd.Function):
         return native.dropout(x.contiguous(), residual.contiguous() if residual is not None else None, cut, rng)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
         (rng,) = ctx.saved_tensors
-        dx = native.dropout(grad.contiguous(), None, ctx.cut, rng) if ctx.needs_input_grad[0] else None
-        return dx, grad if ctx.needs_input_grad[1] else None, None, None
+        want_x, want_residual, _, _ = ctx.needs_input_grad
+        dx = None
+        if want_x and torch.is_grad_enabled():  # a gradient of this gradient is wanted: the operator is linear in x
+            dx = DropoutResidualFunction.apply(grad, None, ctx.cut, rng)
+        elif want_x:
+            dx = native.dropout(grad.contiguous(), None, ctx.cut, rng)
+        return dx, grad if want_residual else None, None, None
 
 
 def dropout_residual(x, p, rng, residual=None):

@@ -38,57 +38,71 @@ class BlockSparseGatedFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, input, weight_data, weight, bias, activation, precision):
-        ctx.weight, ctx.activation, ctx.precision = weight, activation, precision
-        # packed once per forward, never cached: writes through ``.data`` do not bump version counters; backward uses the
-        # weights that the forward saw
-        ctx.packed = weight.packed_weights(precision)
-        if _fused(input, precision):
+        assert weight_data.is_contiguous()
+        ctx.weight, ctx.activation = weight, activation
+        ctx.precision = prec = native.resolve_precision(precision)
+        # The weights are packed once per forward, never cached (writes through ``.data`` do not bump version counters);
+        # backward uses the images made here: the weights that the forward saw.
+        if _fused(input, prec):
             # g and u are kept in bf16, the type of every other tensor that this mode keeps for backward
             h, pre = native.gated_forward(input, _gated_plan(weight), weight_data, bias, activation, True)
+            ctx.packed = native.pack_weights(weight_data, prec).images if ctx.needs_input_grad[0] else None
         else:
-            pre = weight.reverse_matmul(input.float(), transpose=True, bias=bias, packed=ctx.packed)
-            h = native.gated_act(pre, activation, _out_dtype(input, precision))
-        ctx.save_for_backward(input, pre)
+            x = input if input.dtype is torch.float32 else input.float()
+            h, pre, ctx.packed = _gated_pass(weight).forward(x, weight_data, bias, activation, prec, _out_dtype(input, prec))
+        ctx.save_for_backward(input, pre, weight_data)
         return h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        input, pre = ctx.saved_tensors
-        weight = ctx.weight
-        dpre, dbias = native.gated_act_backward(pre, grad.contiguous(), ctx.activation, ctx.needs_input_grad[3])
-        grad_weight = grad_input = None
-        # the weight gradient first, as in BlockSparseLinearFunction: its all-reduce can overlap the input gradient
-        if ctx.needs_input_grad[1]:
-            grad_weight = weight.matmul_with_output_sparse_support(dpre, input, precision=ctx.precision)
-        if ctx.needs_input_grad[0]:
-            grad_input = weight.reverse_matmul(dpre, transpose=False, packed=ctx.packed).to(input.dtype)
-        return grad_input, grad_weight, None, dbias, None, None
+        input, pre, data = ctx.saved_tensors
+        weight, (want_x, want_w, _, want_bias, _, _) = ctx.weight, ctx.needs_input_grad
+        grad = grad.contiguous()
+        if grad.dtype is torch.bfloat16 and (grad.shape[0] < 32 or data.shape[0] == 0):
+            # the products of bf16 tensors start at 32 tokens: fewer go through the fp32 ones
+            grad, pre = grad.float(), pre.float()
+        x = input if input.dtype is grad.dtype else input.to(grad.dtype)
+        dx, dw, dbias, sumsq = _gated_pass(weight).backward(
+            x, pre, grad, data, ctx.packed, ctx.activation, ctx.precision, want_x, want_w, want_bias)
+        if want_w:
+            weight.last_grad_block_sumsq = sumsq
+        return dx if dx is None or dx.dtype is input.dtype else dx.to(input.dtype), dw, None, dbias, None, None
 
 
-def _out_dtype(x, precision):
+def _out_dtype(x, prec):
     """bf16 tensors stay bf16 in the 'bf16' precision; every other combination computes fp32 (as BlockSparseLinear)."""
-    name = native.default_precision() if precision is None else precision
-    return torch.bfloat16 if x.dtype == torch.bfloat16 and name == "bf16" else torch.float32
+    return torch.bfloat16 if x.dtype is torch.bfloat16 and prec == native.PREC_BF16 else torch.float32
 
 
-def _fused(x, precision):
+def _fused(x, prec):
     """Whether the one-kernel forward runs: bf16 tensors in the 'bf16' precision."""
-    return _out_dtype(x, precision) == torch.bfloat16 and x.shape[0] > 0 and x.shape[1] <= native.GATED_MAX_K
+    return prec == native.PREC_BF16 and x.dtype is torch.bfloat16 and x.shape[0] > 0 and x.shape[1] <= native.GATED_MAX_K
+
+
+def _cached_plan(weight, kind, buffers, build):
+    """``build(*buffers)`` kept beside the matrix's other plans while its index buffers are these.  What is built while a
+    stream is captured belongs to the graph and is not kept."""
+    key = (kind, *[v for t in buffers for v in (t.data_ptr(), t._version)])
+    plan = weight._plan_cache.get(key)
+    if plan is None:
+        plan = build(*buffers)
+        if not native.capturing():
+            weight._plan_cache = {k: v for k, v in weight._plan_cache.items() if k[0] != kind}
+            weight._plan_cache[key] = plan
+    return plan
 
 
 def _gated_plan(weight):
-    """Cached per-pattern plan of the one-kernel forward, beside the matrix's other plans."""
-    ptr, idx = weight.row_start_ends_a, weight.cols_a
-    key = ("gated", ptr.data_ptr(), ptr._version, idx.data_ptr(), idx._version)
-    plan = weight._plan_cache.get(key)
-    if plan is None:
-        plan = native.GatedPlan(ptr, idx, weight.shape[0] // 2, weight.shape[1])
-        if native.capturing():
-            return plan
-        weight._plan_cache = {k: v for k, v in weight._plan_cache.items() if k[0] != "gated"}
-        weight._plan_cache[key] = plan
-    return plan
+    """Plan of the one-kernel forward."""
+    return _cached_plan(weight, "gated", (weight.row_start_ends_a, weight.cols_a),
+                        lambda ptr, idx: native.GatedPlan(ptr, idx, weight.shape[0] // 2, weight.shape[1]))
+
+
+def _gated_pass(weight):
+    """Plans of the passes through the matrix's products."""
+    return _cached_plan(weight, "gated pass", (weight.row_start_ends_a, weight.cols_a, weight.col_start_ends_b, weight.rows_b,
+                                               weight.blocks), native.GatedPass)
 
 
 class BlockSparseGatedLinear(nn.Module):
@@ -191,14 +205,14 @@ class BlockSparseGatedLinear(nn.Module):
         return h if len(shape) == 2 else h.reshape(*shape[:-1], self.hidden_features)
 
     def _infer(self, flat, weight, bias, data):
-        out_dtype = _out_dtype(flat, self.precision)
+        prec = native.resolve_precision(self.precision)
         if flat.shape[0] <= SMALL_TOKENS:
             return native.gated_small(flat, weight.row_start_ends_a, weight.cols_a, data, self.hidden_features, bias,
-                                      self.activation, out_dtype)
-        if _fused(flat, self.precision):
+                                      self.activation, _out_dtype(flat, prec))
+        if _fused(flat, prec):
             return native.gated_forward(flat, _gated_plan(weight), data, bias, self.activation, False)[0]
-        pre = weight.reverse_matmul(flat.float(), transpose=True, bias=bias, precision=self.precision)
-        return native.gated_act(pre, self.activation, out_dtype)
+        x = flat if flat.dtype is torch.float32 else flat.float()
+        return _gated_pass(weight).forward(x, data, bias, self.activation, prec, _out_dtype(flat, prec))[0]
 
     def extra_repr(self):
         return "in_features={}, hidden_features={}, bias={}, activation={}, block_count={}".format(

@@ -54,6 +54,9 @@ EXPORTS = (
     "bsmm_gated_act_workspace_bytes",
     "bsmm_gated_act_backward",
     "bsmm_gated_small",
+    "bsmm_gated_pass_forward",
+    "bsmm_gated_backward_workspace_bytes",
+    "bsmm_gated_pass_backward",
     "bsmm_gated_plan_bytes",
     "bsmm_gated_images_bytes",
     "bsmm_build_gated_plan",
@@ -144,6 +147,13 @@ def load():
     lib.bsmm_gated_act_backward.argtypes = [vp, vp, i64, i64, vp, vp, vp, u32, vp]
     lib.bsmm_gated_small.restype = i32
     lib.bsmm_gated_small.argtypes = [vp, i64, i64, vp, vp, i64, vp, i64, vp, vp, u32, vp]
+    lib.bsmm_gated_pass_forward.restype = i32
+    lib.bsmm_gated_pass_forward.argtypes = [vp, i64, i64, vp, vp, i64, vp, vp, vp, i64, vp, vp, vp, u32, vp]
+    lib.bsmm_gated_backward_workspace_bytes.restype = i64
+    lib.bsmm_gated_backward_workspace_bytes.argtypes = [i64, i64, i64, i64, u32]
+    lib.bsmm_gated_pass_backward.restype = i32
+    lib.bsmm_gated_pass_backward.argtypes = [vp, vp, vp, i64, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp,
+                                             vp, u32, vp]
     lib.bsmm_gated_plan_bytes.restype = i64
     lib.bsmm_gated_plan_bytes.argtypes = [i64, i64, i64]
     lib.bsmm_gated_images_bytes.restype = i64
@@ -642,6 +652,71 @@ def gated_act_backward(pre, dh, activation, want_bias):
             "bsmm_gated_act_backward",
         )
     return dpre, dbias
+
+
+class GatedPass:
+    """Forward and backward pass of the gated block through the matrix's products, one library call each
+    (``bsmm_gated_pass_forward``, ``bsmm_gated_pass_backward``), with the plans of one set of index buffers."""
+
+    def __init__(self, ptr, idx, csc_ptr, csc_idx, blocks):
+        self.csr, self.csc = DsdPlan(ptr, idx), DsdPlan(csc_ptr, csc_idx)
+        self.sddmm = SddmmPlan(ptr, idx)
+        self.blocks = _aligned(blocks, 8)
+
+    def forward(self, x, data, bias, activation, precision, out_dtype):
+        """``(h, pre, packed)`` of a contiguous fp32 ``x``: ``pre`` fp32, ``packed`` the weight images (``None``: exact fp32)."""
+        _need_cuda(x, "x")
+        lib, csr, device = load(), self.csr, x.device
+        m, k = x.shape
+        hidden = csr.n_out_blocks * 16
+        pre = torch.empty((m, 2 * hidden), dtype=torch.float32, device=device)
+        h = torch.empty((m, hidden), dtype=out_dtype, device=device)
+        flags = precision | (_gated_flags(activation) | (GATED_IO_BF16 if out_dtype is torch.bfloat16 else 0)) << 16
+        plan = packed = None
+        if precision != PREC_FP32_SIMT:
+            group = csr.group_for(m, precision)
+            plan = csr.buffer(group)
+            flags |= group << 8
+            packed = torch.empty(max(16, lib.bsmm_packed_bytes(csr.nnz, precision)), dtype=torch.uint8, device=device)
+        x, data, bias = _aligned(x), _aligned(data), _aligned(bias)
+        with _on(device):
+            check(
+                lib.bsmm_gated_pass_forward(
+                    x.data_ptr(), m, k, csr.ptr.data_ptr(), csr.idx.data_ptr(), csr.nnz, data.data_ptr(), _ptr(packed), _ptr(plan),
+                    hidden, _ptr(bias), pre.data_ptr(), h.data_ptr(), flags, _stream(device)),
+                "bsmm_gated_pass_forward",
+            )
+        return h, pre, packed
+
+    def backward(self, x, pre, dh, data, packed, activation, precision, want_x, want_w, want_bias):
+        """``(dx, dw, dbias, block_sumsq)``, ``None`` where not wanted; ``x`` and ``dh`` contiguous, of one type."""
+        lib, csc, device = load(), self.csc, dh.device
+        m, hidden = dh.shape
+        k = csc.n_out_blocks * 32
+        dpre = torch.empty((m, 2 * hidden), dtype=dh.dtype, device=device)
+        dx = torch.empty((m, k), dtype=dh.dtype, device=device) if want_x else None
+        dw = torch.empty_like(data) if want_w else None
+        sumsq = torch.empty(csc.nnz, dtype=torch.float32, device=device) if want_w else None
+        dbias = torch.empty(2 * hidden, dtype=torch.float32, device=device) if want_bias else None
+        types = (GATED_IO_BF16 if dh.dtype is torch.bfloat16 else 0) | (GATED_PRE_BF16 if pre.dtype is torch.bfloat16 else 0)
+        flags = precision | (_gated_flags(activation) | types) << 16
+        ws = torch.empty(max(16, lib.bsmm_gated_backward_workspace_bytes(m, k, hidden, csc.nnz, flags)), dtype=torch.uint8, device=device)
+        plan = None
+        if precision != PREC_FP32_SIMT and want_x:
+            group = csc.group_for(m, precision)
+            plan = csc.buffer(group)
+            flags |= group << 8
+        x, dh, data = _aligned(x), _aligned(dh), _aligned(data)
+        with _on(device):
+            check(
+                lib.bsmm_gated_pass_backward(
+                    x.data_ptr(), pre.data_ptr(), dh.data_ptr(), m, k, self.sddmm.idx.data_ptr(), csc.ptr.data_ptr(),
+                    csc.idx.data_ptr(), self.blocks.data_ptr(), csc.nnz, data.data_ptr(), _ptr(packed), _ptr(plan),
+                    self.sddmm.buffer.data_ptr(), hidden, dpre.data_ptr(), _ptr(dx), _ptr(dw), _ptr(dbias), _ptr(sumsq),
+                    ws.data_ptr(), flags, _stream(device)),
+                "bsmm_gated_pass_backward",
+            )
+        return dx, dw, dbias, sumsq
 
 
 def gated_small(x, ptr, idx, data, hidden, bias, activation, out_dtype):

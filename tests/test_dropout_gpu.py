@@ -86,6 +86,16 @@ def test_the_gradient_agrees_with_differences():
     assert abs(diff - (g.double() * v).sum().item()) <= 8 * 2.0 ** -24 * size
 
 
+def test_a_gradient_of_the_gradient():
+    x, v = randn((16, 40), 4).cuda().requires_grad_(), randn((16, 40), 5).cuda().requires_grad_()
+    rng = rng_of(9, 9)
+    (g,) = torch.autograd.grad(dropout_residual(x * x, 0.3, rng), x, v, create_graph=True)  # 2 x v keep / (1 - p)
+    gx, gv = torch.autograd.grad(g.sum(), [x, v])
+    keep = torch.from_numpy(philox_halves(x.numel(), 9, 9) >= round(0.3 * 65536)).view(x.shape).cuda()
+    scale = keep * (65536 / (65536 - round(0.3 * 65536)))
+    assert torch.allclose(gx, 2 * v * scale, rtol=1e-6) and torch.allclose(gv, 2 * x * scale, rtol=1e-6)
+
+
 def test_non_finite_values():
     x = randn((64, 64), 7)
     x[::3, ::2] = float("inf")
