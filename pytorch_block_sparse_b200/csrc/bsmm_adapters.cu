@@ -1,18 +1,18 @@
 // Low-rank adapters of many requests beside a shared projection: out[t] = base[t] + s_a (x[t] D_a^T) U_a^T, where a is the
 // adapter of the request that token t belongs to; tokens of no request, and of requests without an adapter, keep base[t].
 //
-// Two launches: the shrink kernel writes v[t] = x[t] D_a^T in fp32 (partial sums over ranges of the input features when
-// few tokens would leave SMs idle), the expand kernel adds the partial sums in order, scales and multiplies by U_a.
-// Both are memory bound and work with mma.sync on fragments of 16 bytes per lane.  The contraction index of such a product
-// may be permuted as long as both operands agree, so a lane takes eight CONSECUTIVE k of its row -- what two (bf16) or four
-// (tf32) instructions want from it -- and the output columns of four instructions are permuted the same way, so that a
-// lane ends with eight consecutive columns of each of its two rows.
+// Memory bound: work goes through mma.sync on fragments of 16 bytes per lane.  The contraction index of such a product may be
+// permuted as long as both operands agree, so a lane takes eight CONSECUTIVE k of its row -- what two (bf16) or four (tf32)
+// instructions want from it -- and the output columns of four instructions are permuted the same way, so that a lane ends
+// with eight consecutive columns of each of its two rows.
 //
-// Two forms of each kernel, chosen by the average number of tokens per request:
-//   warps   (few tokens per request) a warp owns 16 tokens and walks the distinct adapters among them on its own, fragments
-//           straight from global memory; with many short requests the walk is shared between `subs` warps
-//   tiles   (prompts) a CTA owns 128 tokens and walks their adapters; the adapter's matrix passes through shared memory
-//           once for its eight warps, where the first form reads it once per 16 tokens
+// Two forms, chosen by the average number of tokens per request:
+//   clusters  (few tokens per request) one launch: a cluster of eight CTAs owns 4 or 16 tokens.  Each CTA takes an eighth of the
+//             input features for v[t] = x[t] D_a^T, the partial v are exchanged through distributed shared memory, and
+//             each CTA writes an eighth of the outputs.  Inside a CTA the warps share the tile's distinct adapters and the
+//             features; fragments come straight from global memory
+//   tiles     (prompts) two launches: the shrink kernel writes v, the expand kernel multiplies by U_a.  A CTA owns 128 tokens
+//             of one request; the adapter's matrix passes through shared memory once for its eight warps
 //
 // Arithmetic.  fp32 tensors: both operands are split into tf32 hi + lo parts and three products are added (about 2^-21
 // relative per term); bf16 tensors: x D is one exact product, v is split into bf16 hi + lo (its rounding to one bf16 would
@@ -28,8 +28,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kTokens = 16;       // tokens of a warp
-constexpr int kWarps = 4;         // warps of a CTA, each on its own
 constexpr int kStep = 32;         // input features of one step
 constexpr int kNone = -1;
 
@@ -164,102 +162,40 @@ __device__ __forceinline__ void load_pieces(Fragment<float, kLen>& f, const uint
 __device__ __forceinline__ void wait_for_shrink() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_expand_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// The adapter of token t, or kNone.  Offsets and ids come from the device unchecked: whatever they hold, the search stays
-// inside the arrays and ends, and an id outside [0, count) counts as none.
-__device__ __forceinline__ int adapter_of(int64_t t, int64_t tokens, const int32_t* __restrict__ offsets,
-                                          const int32_t* __restrict__ ids, int requests, int count) {
-    if (t >= tokens || requests == 0) return kNone;
-    int lo = 0, hi = requests;  // first request whose end lies behind t
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(offsets + mid + 1) <= t) lo = mid + 1; else hi = mid;
+// ids[i] = adapter of token t0 + i, or kNone, for i < count <= 16; by one warp.  Offsets and ids come from the device
+// unchecked: whatever they hold, the search stays inside the arrays and ends, and an id outside [0, count) counts as none.
+// 32 requests are looked at per step, so that the usual batch costs two dependent loads where a binary search costs seven.
+__device__ __forceinline__ void find_adapters(const AdapterCall& p, int64_t t0, int count, int* ids) {
+    const int lane = threadIdx.x & 31, n = (int)p.requests;
+    if (lane < count) ids[lane] = kNone;
+    int lo = 0, hi = n;  // the first request that ends behind t0 lies in [lo, hi]
+    while (hi - lo > 32) {
+        const int step = (hi - lo + 31) / 32, probe = lo + (lane + 1) * step - 1;
+        const bool before = probe < hi && __ldg(p.offsets + probe + 1) <= t0;
+        const int c = __popc(__ballot_sync(0xffffffffu, before));
+        const int from = min(hi, lo + c * step);
+        hi = min(hi, from + step);
+        lo = from;
     }
-    if (lo == requests || __ldg(offsets + lo) > t) return kNone;
-    const int id = __ldg(ids + lo);
-    return id >= 0 && id < count ? id : kNone;
-}
-
-struct Units {
-    int64_t tiles;      // of kTokens tokens
-    int64_t parts;      // ranges of input features (shrink) or of output features (expand)
-    int subs;           // warps that share a tile's adapters
-    int64_t per_part;   // features of a part, a multiple of 32
-};
-
-// ------------------------------------------------------------------------------------------------ a warp on its own
-// v[split][t][0 .. rank) = sum over the split's input features of x[t] D_a^T
-template <typename T, int kRank>  // kRank rows of D at a time: 16, 32 or 64
-__global__ void __launch_bounds__(32 * kWarps)
-shrink_kernel(AdapterCall p, Units units) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    let_expand_start();
-    if (unit >= units.tiles * units.parts * units.subs) return;
-    const int64_t tile = unit % units.tiles, rest = unit / units.tiles;
-    const int sub = (int)(rest % units.subs);
-    const int64_t part = rest / units.subs;
-    const int64_t k0 = part * units.per_part, k1 = min(p.inner, k0 + units.per_part);
-    const int64_t t0 = tile * kTokens;
-    const T* x = static_cast<const T*>(p.x);
-
-    const int mine = lane < kTokens ? adapter_of(t0 + lane, p.tokens, p.offsets, p.ids, (int)p.requests, (int)p.count) : kNone;
-    uint32_t todo = __ballot_sync(0xffffffffu, mine != kNone);
-    const bool live0 = t0 + g < p.tokens, live1 = t0 + g + 8 < p.tokens;
-    for (int turn = 0; todo != 0; ++turn) {
-        const int id = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
-        const uint32_t rows = __ballot_sync(0xffffffffu, mine == id);
-        todo &= ~rows;
-        if (turn % units.subs != sub) continue;
-        for (int64_t r0 = 0; r0 < p.rank; r0 += kRank) {
-            const T* down = static_cast<const T*>(p.down) + ((int64_t)id * p.rank + r0) * p.inner;
-            float acc[kRank / 8][4];
-#pragma unroll
-            for (int n = 0; n < kRank / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-#pragma unroll 2
-            for (int64_t k = k0 + q * 8; k < k1; k += kStep) {
-                Fragment<T, 8> a0, a1;
-                if (live0) a0.load(x + (t0 + g) * p.inner + k); else a0.clear();
-                if (live1) a1.load(x + (t0 + g + 8) * p.inner + k); else a1.clear();
-#pragma unroll
-                for (int n0 = 0; n0 < kRank / 8; n0 += 2) {
-                    Fragment<T, 8> b[2];
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) b[n].load(down + (int64_t)((n0 + n) * 8 + g) * p.inner + k);
-                    multiply<8, 2>(acc + n0, a0, a1, b);
-                }
-            }
-            float* v = p.workspace + (part * p.tokens + t0) * p.rank + r0 + 2 * q;
-#pragma unroll
-            for (int n = 0; n < kRank / 8; ++n) {
-                if ((rows >> g) & 1u) *reinterpret_cast<float2*>(v + g * p.rank + n * 8) = make_float2(acc[n][0], acc[n][1]);
-                if ((rows >> (g + 8)) & 1u)
-                    *reinterpret_cast<float2*>(v + (g + 8) * p.rank + n * 8) = make_float2(acc[n][2], acc[n][3]);
-            }
+    __syncwarp();
+    const int64_t t1 = min(t0 + count, p.tokens);
+    for (bool more = true; more && lo < n; lo += 32) {
+        const int r = lo + lane;
+        int64_t start = 0, end = 0;
+        int id = kNone;
+        if (r < n) {
+            start = __ldg(p.offsets + r);
+            end = __ldg(p.offsets + r + 1);
+            id = __ldg(p.ids + r);
+            if (id < 0 || id >= p.count) id = kNone;
         }
+        for (int64_t t = max(start, t0); t < min(end, t1); ++t) ids[t - t0] = id;
+        more = !__any_sync(0xffffffffu, r < n && end >= t1);
     }
+    __syncwarp();
 }
 
-// the values of v that a lane holds as an operand: kLen of token t from r on, summed over the splits and scaled
-template <typename T, int kLen>
-__device__ __forceinline__ void load_v(const AdapterCall& p, int64_t splits, int64_t t, int64_t r, float scale, bool wanted,
-                                       SplitFragment<T, kLen>& f) {
-    float v[kLen];
-#pragma unroll
-    for (int i = 0; i < kLen; ++i) v[i] = 0.f;
-    if (wanted) {
-        for (int64_t s = 0; s < splits; ++s) {
-            const float4* src = reinterpret_cast<const float4*>(p.workspace + (s * p.tokens + t) * p.rank + r);
-#pragma unroll
-            for (int i = 0; i < kLen / 4; ++i) {
-                const float4 w = src[i];
-                v[4 * i] += w.x; v[4 * i + 1] += w.y; v[4 * i + 2] += w.z; v[4 * i + 3] += w.w;
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kLen; ++i) v[i] *= scale;
-    f.set(v);
-}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 template <typename O>
 __device__ __forceinline__ void add_base_and_store(const AdapterCall& p, int64_t t, int64_t n, float (&v)[8]) {
@@ -273,54 +209,159 @@ __device__ __forceinline__ void add_base_and_store(const AdapterCall& p, int64_t
     store8(static_cast<O*>(p.out) + t * p.outer + n, v);
 }
 
-template <typename T, typename O, int kRank>
-__global__ void __launch_bounds__(32 * kWarps)
-expand_kernel(AdapterCall p, Units units, int64_t splits) {
+// ------------------------------------------------------------------------------------------ a cluster on 4 or 16 tokens
+constexpr int kClusterCtas = 8, kClusterWarps = 8, kClusterRows = 16;
+
+// dynamic shared memory: [8 warps][16][kRank] partial sums of a round, [16][rank + 4] this CTA's v, the same of the cluster's
+template <int kRank>
+constexpr int cluster_smem(int64_t rank) {
+    return (kClusterWarps * kClusterRows * kRank + 2 * kClusterRows * ((int)rank + 4)) * 4;
+}
+
+template <typename T, typename O, int kRank>  // kRank rows of D at a time: 16, 32 or 64
+__global__ void __launch_bounds__(32 * kClusterWarps)
+cluster_kernel(AdapterCall p, int tile_tokens, int64_t in_part, int64_t out_part) {
     constexpr int kLen = kRank == 16 ? 4 : 8;            // a lane's values of one load: 16 or 32 of the rank per warp load
     constexpr int kLoads = kRank / (4 * kLen);
-    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (unit >= units.tiles * units.parts * units.subs) {
-        wait_for_shrink();
-        return;
-    }
-    const int64_t tile = unit % units.tiles, rest = unit / units.tiles;
-    const int sub = (int)(rest % units.subs);
-    const int64_t part = rest / units.subs;
-    const int64_t n0 = part * units.per_part, n1 = min(p.outer, n0 + units.per_part);
-    const int64_t t0 = tile * kTokens;
+    extern __shared__ __align__(16) float csmem[];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const int cta = (int)(blockIdx.x % kClusterCtas);
+    const int64_t t0 = (int64_t)(blockIdx.x / kClusterCtas) * tile_tokens;
+    const int pitch = (int)p.rank + 4;
+    float* parts = csmem;
+    float* own = parts + kClusterWarps * kClusterRows * kRank;
+    float* total = own + kClusterRows * pitch;
 
-    const int mine = lane < kTokens ? adapter_of(t0 + lane, p.tokens, p.offsets, p.ids, (int)p.requests, (int)p.count) : kNone;
-    uint32_t todo = __ballot_sync(0xffffffffu, mine != kNone);
-    const uint32_t idle = ~todo & 0xFFFFu;  // tokens without an adapter keep their base
-    if (sub == 0 && (p.base != p.out)) {
-        for (int row = g; row < kTokens; row += 8) {
-            if (!((idle >> row) & 1u) || t0 + row >= p.tokens) continue;
-            for (int64_t n = n0 + q * 8; n < n1; n += 32) {
+    // every warp knows the adapter of each of the tile's tokens: lane i holds token i's
+    __shared__ int ids[kClusterRows];
+    if (warp == 0) find_adapters(p, t0, tile_tokens, ids);
+    __syncthreads();
+    const int mine = lane < tile_tokens ? ids[lane] : kNone;
+    const uint32_t all = __ballot_sync(0xffffffffu, mine != kNone);
+    // distinct adapters: those at their first token
+    const uint32_t alike = __match_any_sync(0xffffffffu, mine);
+    const uint32_t leaders = __ballot_sync(0xffffffffu, mine != kNone && (int)(__ffs(alike) - 1) == lane);
+    const int distinct = __popc(leaders);
+    // the warps share the adapters, then each adapter's features
+    const int subs = distinct >= 4 ? 4 : distinct >= 2 ? 2 : 1, shares = kClusterWarps / subs;
+    const int sub = warp % subs, share = warp / subs;
+
+    const T* x = static_cast<const T*>(p.x);
+    const int64_t row0 = t0 + g, row1 = t0 + g + 8;
+    const bool live0 = g < tile_tokens && row0 < p.tokens, live1 = g + 8 < tile_tokens && row1 < p.tokens;
+    const int64_t begin = min(p.outer, cta * out_part), end = min(p.outer, begin + out_part);
+    const int64_t each = (end - begin + 32 * shares - 1) / (32 * shares) * 32;
+    const int64_t n0 = min(end, begin + share * each), n1 = min(end, n0 + each);
+    {   // what the second half will read of U is asked for now
+        uint32_t todo = leaders;
+        for (int turn = 0; todo != 0; ++turn, todo &= todo - 1) {
+            if (turn % subs != sub) continue;
+            const int id = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
+            const char* up = reinterpret_cast<const char*>(static_cast<const T*>(p.up) + ((int64_t)id * p.outer + n0) * p.rank);
+            const int64_t bytes = (n1 - n0) * p.rank * (int64_t)sizeof(T);
+            for (int64_t at = lane * 128; at < bytes; at += 32 * 128) prefetch_l2(up + at);
+        }
+    }
+    {
+        const int64_t begin = min(p.inner, cta * in_part), end = min(p.inner, begin + in_part);
+        const int64_t each = (end - begin + kStep * shares - 1) / (kStep * shares) * kStep;
+        const int64_t k0 = min(end, begin + share * each), k1 = min(end, k0 + each);
+        for (int64_t r0 = 0; r0 < p.rank; r0 += kRank) {
+            uint32_t todo = leaders;
+            for (int turn = 0; todo != 0; ++turn, todo &= todo - 1) {
+                if (turn % subs != sub) continue;
+                const int id = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
+                const uint32_t rows = __shfl_sync(0xffffffffu, alike, __ffs(todo) - 1);
+                const T* down = static_cast<const T*>(p.down) + ((int64_t)id * p.rank + r0) * p.inner;
+                float acc[kRank / 8][4];
+#pragma unroll
+                for (int n = 0; n < kRank / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+#pragma unroll 4
+                for (int64_t k = k0 + q * 8; k < k1; k += kStep) {
+                    Fragment<T, 8> a0, a1;
+                    if (live0) a0.load(x + row0 * p.inner + k); else a0.clear();
+                    if (live1) a1.load(x + row1 * p.inner + k); else a1.clear();
+#pragma unroll
+                    for (int n0 = 0; n0 < kRank / 8; n0 += 2) {
+                        Fragment<T, 8> b[2];
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) b[n].load(down + (int64_t)((n0 + n) * 8 + g) * p.inner + k);
+                        multiply<8, 2>(acc + n0, a0, a1, b);
+                    }
+                }
+                float* to = parts + share * kClusterRows * kRank + 2 * q;
+#pragma unroll
+                for (int n = 0; n < kRank / 8; ++n) {
+                    if ((rows >> g) & 1u) *reinterpret_cast<float2*>(to + g * kRank + n * 8) = make_float2(acc[n][0], acc[n][1]);
+                    if ((rows >> (g + 8)) & 1u)
+                        *reinterpret_cast<float2*>(to + (g + 8) * kRank + n * 8) = make_float2(acc[n][2], acc[n][3]);
+                }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < tile_tokens * kRank; i += 32 * kClusterWarps) {
+                const int row = i / kRank, r = i % kRank;
+                if (!((all >> row) & 1u)) continue;
+                float sum = 0.f;
+                for (int s = 0; s < shares; ++s) sum += parts[(s * kClusterRows + row) * kRank + r];
+                own[row * pitch + r0 + r] = sum;
+            }
+            __syncthreads();
+        }
+    }
+    cluster.sync();
+    {
+        // the cluster's sums, in the CTAs' order, scaled by the token's adapter
+        const int rank = (int)p.rank;
+        for (int i = threadIdx.x; i < tile_tokens * rank / 4; i += 32 * kClusterWarps) {
+            const int row = i * 4 / rank, r = i * 4 % rank;
+            if (!((all >> row) & 1u)) continue;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < kClusterCtas; ++c) {
+                const float4 w = *reinterpret_cast<const float4*>(cluster.map_shared_rank(own, c) + row * pitch + r);
+                sum.x += w.x; sum.y += w.y; sum.z += w.z; sum.w += w.w;
+            }
+            const float scale = __ldg(p.scaling + ids[row]);
+            *reinterpret_cast<float4*>(total + row * pitch + r) = make_float4(sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale);
+        }
+    }
+    cluster.barrier_arrive();  // this CTA has read the others' sums
+    __syncthreads();
+    if (p.base != p.out) {  // tokens without an adapter keep their base
+        for (int row = warp; row < tile_tokens; row += kClusterWarps) {
+            if (((all >> row) & 1u) || t0 + row >= p.tokens) continue;
+#pragma unroll 2
+            for (int64_t n = begin + lane * 8; n < end; n += 256) {
                 float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                 add_base_and_store<O>(p, t0 + row, n, v);
             }
         }
     }
-    wait_for_shrink();
-    for (int turn = 0; todo != 0; ++turn) {
+    uint32_t todo = leaders;
+    for (int turn = 0; todo != 0; ++turn, todo &= todo - 1) {
+        if (turn % subs != sub) continue;
         const int id = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
-        const uint32_t rows = __ballot_sync(0xffffffffu, mine == id);
-        todo &= ~rows;
-        if (turn % units.subs != sub) continue;
-        const bool row0 = ((rows >> g) & 1u) != 0, row1 = ((rows >> (g + 8)) & 1u) != 0;
-        const float scale = __ldg(p.scaling + id);
+        const uint32_t rows = __shfl_sync(0xffffffffu, alike, __ffs(todo) - 1);
+        const bool use0 = ((rows >> g) & 1u) != 0, use1 = ((rows >> (g + 8)) & 1u) != 0;
         const T* up = static_cast<const T*>(p.up) + (int64_t)id * p.outer * p.rank;
         SplitFragment<T, kLen> v0[kLoads], v1[kLoads];
-        auto load_rank = [&](int64_t r0) {
+        auto load_rank = [&](int64_t r0) {  // (rows of other adapters are computed along and not stored)
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int64_t r = r0 + (i * 4 + q) * kLen;
-                load_v<T, kLen>(p, splits, t0 + g, r, scale, row0, v0[i]);
-                load_v<T, kLen>(p, splits, t0 + g + 8, r, scale, row1, v1[i]);
+                float a[kLen], b[kLen];
+                const float* from = total + g * pitch + r0 + (i * 4 + q) * kLen;
+#pragma unroll
+                for (int e = 0; e < kLen; e += 4) {
+                    *reinterpret_cast<float4*>(a + e) = *reinterpret_cast<const float4*>(from + e);
+                    *reinterpret_cast<float4*>(b + e) = *reinterpret_cast<const float4*>(from + 8 * pitch + e);
+                }
+                v0[i].set(a);
+                v1[i].set(b);
             }
         };
         if (p.rank == kRank) load_rank(0);
+#pragma unroll 4
         for (int64_t n = n0; n < n1; n += 32) {
             float acc[4][4];
 #pragma unroll
@@ -340,17 +381,24 @@ expand_kernel(AdapterCall p, Units units, int64_t splits) {
                         multiply<kLen, kGroup<T>>(acc + j0, v0[i], v1[i], b);
                     }
             }
-            if (row0) {
+            if (use0) {
                 float v[8] = {acc[0][0], acc[0][1], acc[1][0], acc[1][1], acc[2][0], acc[2][1], acc[3][0], acc[3][1]};
-                add_base_and_store<O>(p, t0 + g, n + q * 8, v);
+                add_base_and_store<O>(p, row0, n + q * 8, v);
             }
-            if (row1) {
+            if (use1) {
                 float v[8] = {acc[0][2], acc[0][3], acc[1][2], acc[1][3], acc[2][2], acc[2][3], acc[3][2], acc[3][3]};
-                add_base_and_store<O>(p, t0 + g + 8, n + q * 8, v);
+                add_base_and_store<O>(p, row1, n + q * 8, v);
             }
         }
     }
+    cluster.barrier_wait();  // nobody leaves while its sums are read
 }
+
+struct Units {
+    int64_t tiles;      // of 128 tokens
+    int64_t parts;      // ranges of input features (shrink) or of output features (expand)
+    int64_t per_part;   // features of a part, a multiple of 32
+};
 
 // ---------------------------------------------------------------------------------------------- a CTA on 128 tokens
 constexpr int kTileTokens = 128, kTileWarps = 8, kTileThreads = 32 * kTileWarps;
@@ -696,44 +744,19 @@ expand_tile_kernel(AdapterCall p, Units units) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int64_t kWantedWarps = 148 * 8;
-
-// Prompts go by tiles of 128 tokens, short requests by warps of 16: TILES_NOTE
+// Prompts go by tiles of 128 tokens, short requests by clusters: TILES_NOTE
 bool by_tiles(int64_t tokens, int64_t requests) { return tokens >= 256 && tokens >= 32 * requests; }
 
-// How the input features are cut: enough warps to fill the GPU, at least 128 features each, at most 16 partial sums.
-Units shrink_units(int64_t tokens, int64_t inner) {
-    Units u;
-    u.tiles = ceil_div(tokens, kTokens);
-    u.subs = 1;
-    int64_t parts = ceil_div(kWantedWarps, u.tiles);
-    parts = parts < 16 ? parts : 16;
-    const int64_t most = ceil_div(inner, 128);
-    parts = parts < most ? parts : most;
-    u.per_part = ceil_div(ceil_div(inner, parts), 32) * 32;
-    u.parts = ceil_div(inner, u.per_part);
-    return u;
-}
-
-// The same for tiles: CTAs of a cluster (a power of two up to 8), two per SM, at least 256 features each.  Tiles start at each
-// request's start, so that there may be one more for every request and for the tokens around them; half that is expected.
+// How the input features are cut: CTAs of a cluster (a power of two up to 8), two per SM, at least 256 features each.  Tiles
+// start at each request's start, so that there may be one more for every request and for the tokens around them; half that is expected.
 Units tile_units(const AdapterCall& p) {
     Units u;
     u.tiles = ceil_div(p.tokens, kTileTokens) + p.requests + 2;
-    u.subs = 1;
     const int64_t expected = ceil_div(p.tokens, kTileTokens) + p.requests / 2;
     u.parts = 1;
     while (u.parts < 8 && expected * u.parts * 2 <= 2 * 148 && u.parts * 2 * 256 <= p.inner) u.parts *= 2;
     u.per_part = ceil_div(ceil_div(p.inner, u.parts), 64) * 64;
     return u;
-}
-
-// Distinct adapters a warp's 16 tokens may hold: as many as the requests that meet in it, on average.
-int sub_count(const AdapterCall& p) {
-    const int64_t meet = ceil_div(kTokens * p.requests, p.tokens);
-    int subs = 1;
-    while (subs < meet && subs < kTokens) subs *= 2;
-    return subs;
 }
 
 // A launch in clusters of `cluster` CTAs, or one that may begin while the kernel before it still runs.
@@ -802,14 +825,14 @@ cudaError_t launch_tiles(const AdapterCall& p, cudaStream_t stream) {
 template <typename T, typename O, int kRank>
 cudaError_t launch(const AdapterCall& p, cudaStream_t stream) {
     if (by_tiles(p.tokens, p.requests)) return launch_tiles<T, O, kRank>(p, stream);
-    Units shrink = shrink_units(p.tokens, p.inner), expand = shrink;
-    shrink.subs = expand.subs = sub_count(p);
-    cut_outputs(expand, p.outer, 32, ceil_div(kWantedWarps * 2, expand.tiles * expand.subs));
-    const cudaError_t err = launch_with(shrink_kernel<T, kRank>, ceil_div(shrink.tiles * shrink.parts * shrink.subs, kWarps),
-                                        32 * kWarps, 0, 1, false, stream, p, shrink);
+    static bool ready[64] = {false};
+    const cudaError_t err = allow_smem(cluster_kernel<T, O, kRank>, cluster_smem<kRank>(kRank < 64 ? kRank : 256), ready);
     if (err != cudaSuccess) return err;
-    return launch_with(expand_kernel<T, O, kRank>, ceil_div(expand.tiles * expand.parts * expand.subs, kWarps), 32 * kWarps, 0, 1,
-                       true, stream, p, expand, shrink.parts);
+    // few tokens: smaller tiles, more CTAs
+    const int tile_tokens = ceil_div(p.tokens, 4) * kClusterCtas <= 2 * 148 ? 4 : kClusterRows;
+    const int64_t in_part = ceil_div(p.inner, kClusterCtas * 32) * 32, out_part = ceil_div(p.outer, kClusterCtas * 32) * 32;
+    return launch_with(cluster_kernel<T, O, kRank>, ceil_div(p.tokens, tile_tokens) * kClusterCtas, 32 * kClusterWarps,
+                       cluster_smem<kRank>(p.rank), kClusterCtas, false, stream, p, tile_tokens, in_part, out_part);
 }
 
 template <typename T, typename O>
@@ -824,7 +847,8 @@ cudaError_t by_rank(const AdapterCall& p, cudaStream_t stream) {
 
 int64_t adapters_workspace_bytes(int64_t tokens, int64_t inner, int64_t rank) {
     if (tokens == 0) return 0;
-    return shrink_units(tokens, inner).parts * tokens * rank * (int64_t)sizeof(float);  // (tiles: one sum only)
+    (void)inner;
+    return tokens * rank * (int64_t)sizeof(float);  // v
 }
 
 cudaError_t launch_adapters(const AdapterCall& p, bool in_bf16, bool out_bf16, cudaStream_t stream) {
