@@ -744,8 +744,10 @@ expand_tile_kernel(AdapterCall p, Units units) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Prompts go by tiles of 128 tokens, short requests by clusters: TILES_NOTE
-bool by_tiles(int64_t tokens, int64_t requests) { return tokens >= 256 && tokens >= 32 * requests; }
+// Prompts go by tiles of 128 tokens, short requests and small batches by clusters.  us at 4096 -> 4096 features, rank 64,
+// clusters / tiles: 512 tokens in 2 requests 15 / 18, in 16 requests 15 / 19; 1024 tokens in 4 requests 29 / 20, in 32 29 / 28, in
+// 64 30 / 37; 4096 tokens in 64 requests 117 / 47, in 128 117 / 84, in 256 117 / 109 (rank 16: 66 / 29, 66 / 50, 66 / 71).
+bool by_tiles(int64_t tokens, int64_t requests) { return tokens >= 768 && tokens >= 32 * requests; }
 
 // How the input features are cut: CTAs of a cluster (a power of two up to 8), two per SM, at least 256 features each.  Tiles
 // start at each request's start, so that there may be one more for every request and for the tokens around them; half that is expected.

@@ -66,6 +66,8 @@ MIXES = {
     "some without": ([5, 7, 0, 40, 1], [None, 3, 1, None, 0]),
     "none at all": ([4, 9], [None, None]),
     "a prompt among tokens": ([1, 1, 1, 200, 1, 1], [4, 3, 2, 1, 0, 4]),
+    "a prompt of many clusters": ([300, 7], [1, 3]),
+    "more requests than a warp asks for at once": ([1, 0, 2] * 60, [i % 5 for i in range(180)]),
 }
 
 
@@ -96,10 +98,11 @@ def run_mix(lengths, ids, types, sizes):
 
 
 PROMPTS = {  # long enough for the form that owns 128 tokens at a time
-    "one": ([256], [1]),
-    "odd": ([257, 130, 0, 1, 3, 129], [0, 3, 1, 2, None, 4]),
-    "many adapters in a tile": ([500, 5, 1, 7, 2, 30, 1, 60], [0, 1, 2, 3, 4, 0, 1, 2]),
-    "none but one": ([300, 20, 300], [None, 4, None]),
+    "one": ([769], [1]),
+    "odd": ([577, 130, 0, 1, 3, 129], [0, 3, 1, 2, None, 4]),
+    "many adapters near one another": ([700, 5, 1, 7, 2, 30, 1, 60], [0, 1, 2, 3, 4, 0, 1, 2]),
+    "none but one": ([400, 20, 400], [None, 4, None]),
+    "more requests than a warp asks for at once": ([40] * 70, [i % 6 - 1 for i in range(70)]),
 }
 
 
@@ -134,12 +137,12 @@ def test_tokens_outside_every_request_keep_their_base():
         alone = ad(x.cuda(), requests).cpu()
         assert (alone[:3] == 0).all() and (alone[40:] == 0).all()
         # the same for long prompts
-        xl, bl = randn((600, 64), 3), randn((600, 64), 4)
-        xl[:3], xl[570:] = float("inf"), float("nan")
-        long = AdapterRequests(torch.tensor([3, 300, 570], dtype=torch.int32, device="cuda"), torch.tensor([1, 0], dtype=torch.int32, device="cuda"))
+        xl, bl = randn((900, 64), 3), randn((900, 64), 4)
+        xl[:3], xl[870:] = float("inf"), float("nan")
+        long = AdapterRequests(torch.tensor([3, 300, 870], dtype=torch.int32, device="cuda"), torch.tensor([1, 0], dtype=torch.int32, device="cuda"))
         got = ad(xl.cuda(), long, base=bl.cuda()).cpu()
-        assert torch.equal(got[:3], bl[:3]) and torch.equal(got[570:], bl[570:])
-        check(got[3:570], xl[3:570], [297, 270], [1, 0], weights, bl[3:570], torch.float32, 64, 16)
+        assert torch.equal(got[:3], bl[:3]) and torch.equal(got[870:], bl[870:])
+        check(got[3:870], xl[3:870], [297, 570], [1, 0], weights, bl[3:870], torch.float32, 64, 16)
         # a token's NaN stays its own
         x2 = randn((50, 64), 1)
         x2[20] = float("nan")
