@@ -333,7 +333,11 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
  *   flags                      precision, BSMM_DSD_GROUP(g) of `plan` (forward) or `csc_plan` (backward),
  *                              BSMM_GATED_PASS(activation and type flags as for bsmm_gated_act)
  *   dx, dw, dbias              NULL where not wanted; block_sumsq as bsmm_sddmm
- *   workspace                  bsmm_gated_backward_workspace_bytes bytes, 16-byte aligned
+ *   wgrad_plan                 bsmm_build_gated_wgrad_plan of the CSR, bsmm_gated_wgrad_plan_bytes bytes, 16-byte aligned, or NULL: with
+ *                              it the weight gradient of fp32 tensors in BSMM_PREC_TF32X3 and BSMM_PREC_BF16X3 (64 tokens or more)
+ *                              comes from a kernel that multiplies three bf16 parts of every value and shares the input
+ *                              between gate and up blocks (relative error near 1e-6), else from bsmm_sddmm
+ *   workspace                  bsmm_gated_backward_workspace_bytes bytes, 256-byte aligned
  */
 #define BSMM_GATED_PASS(f) (((uint32_t)(f)&0xFu) << 16)
 int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, int64_t nnz,
@@ -343,8 +347,11 @@ int64_t bsmm_gated_backward_workspace_bytes(int64_t m, int64_t k, int64_t hidden
 int bsmm_gated_pass_backward(const void* x, const void* pre, const void* dh, int64_t m, int64_t k, const int32_t* idx,
                              const int32_t* csc_ptr, const int32_t* csc_idx, const int32_t* blocks, int64_t nnz,
                              const float* data, const void* packed, const void* csc_plan, const void* sddmm_plan,
-                             int64_t hidden, void* dpre, void* dx, float* dw, float* dbias, float* block_sumsq,
-                             void* workspace, uint32_t flags, bsmm_stream_t stream);
+                             const void* wgrad_plan, int64_t hidden, void* dpre, void* dx, float* dw, float* dbias,
+                             float* block_sumsq, void* workspace, uint32_t flags, bsmm_stream_t stream);
+int64_t bsmm_gated_wgrad_plan_bytes(int64_t hidden, int64_t k, int64_t nnz);
+int bsmm_build_gated_wgrad_plan(const int32_t* ptr, const int32_t* idx, int64_t hidden, int64_t k, int64_t nnz, void* plan,
+                                bsmm_stream_t stream);
 
 /*
  * The gated block on bf16 tensors with bf16 products (fp32 sums) in one tensor-core kernel: both projections, the activation

@@ -46,6 +46,34 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
         make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
+// w = parts[0] + parts[1] + parts[2] exactly (3 x 8 significant bits), for a pair of values
+__device__ __forceinline__ void split3_bf16x2(float w0, float w1, uint32_t (&parts)[3]) {
+    asm("{\n\t.reg .b16 h0, h1, m1;\n\t.reg .f32 d0, d1;\n\t"
+        "mov.b16 m1, 0xBF80;\n\t"
+        "cvt.rn.bf16x2.f32 %0, %4, %3;\n\t"
+        "mov.b32 {h0, h1}, %0;\n\t"
+        "fma.rn.f32.bf16 d0, h0, m1, %3;\n\t"
+        "fma.rn.f32.bf16 d1, h1, m1, %4;\n\t"
+        "cvt.rn.bf16x2.f32 %1, d1, d0;\n\t"
+        "mov.b32 {h0, h1}, %1;\n\t"
+        "fma.rn.f32.bf16 d0, h0, m1, d0;\n\t"
+        "fma.rn.f32.bf16 d1, h1, m1, d1;\n\t"
+        "cvt.rn.bf16x2.f32 %2, d1, d0;\n\t}"
+        : "=&r"(parts[0]), "=&r"(parts[1]), "=r"(parts[2])
+        : "f"(w0), "f"(w1));
+}
+
+// Planes: an fp32 matrix [tokens][features] as three bf16 matrices [features][pitch] that add up to it exactly.
+__host__ __device__ constexpr int64_t plane_pitch(int64_t tokens) { return (tokens + 7) / 8 * 8; }  // rows of whole 16-byte pieces
+// eight consecutive tokens of a feature to the three planes, `plane` elements apart
+__device__ __forceinline__ void store_planes(const float* v, __nv_bfloat16* to, int64_t plane) {
+    uint32_t parts[4][3];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split3_bf16x2(v[2 * j], v[2 * j + 1], parts[j]);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(to + q * plane) = make_uint4(parts[0][q], parts[1][q], parts[2][q], parts[3][q]);
+}
+
 // the same as loaded, not yet widened: what a thread holds while loads are in flight
 template <typename T>
 struct Raw8;
@@ -101,7 +129,7 @@ cudaError_t launch_gated_act(const void* pre, int64_t m, int64_t hidden, void* h
 int64_t gated_act_workspace_bytes(int64_t m, int64_t hidden);
 cudaError_t launch_gated_act_backward(const void* pre, const void* dh, int64_t m, int64_t hidden, void* dpre,
                                       float* dbias, float* workspace, int act, bool pre_bf16, bool io_bf16,
-                                      cudaStream_t stream);
+                                      void* planes, cudaStream_t stream);  // planes of dpre, or null (fp32 only)
 cudaError_t launch_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx,
                                const float* data, int64_t nnz, int64_t hidden, const float* bias, void* h, int act,
                                bool x_bf16, bool h_bf16, cudaStream_t stream);
@@ -115,6 +143,15 @@ cudaError_t launch_pack_pairs(const float* data, const void* plan, int64_t hidde
                               cudaStream_t stream);
 cudaError_t launch_gated_umma(const void* x, int64_t m, int64_t k, const void* plan, const void* images, int64_t hidden,
                               const float* bias, void* h, void* pre, int act, cudaStream_t stream);
+
+// the weight gradient of fp32 tensors from planes of three bf16 parts (bsmm_gated_wgrad.cu)
+int64_t gated_wgrad_plan_bytes(int64_t hidden, int64_t nnz);
+cudaError_t launch_build_gated_wgrad_plan(const int32_t* ptr, const int32_t* idx, int64_t hidden, int64_t k, int64_t nnz, void* plan,
+                                          cudaStream_t stream);
+cudaError_t launch_split_planes(const float* x, int64_t m, int64_t k, void* planes, cudaStream_t stream);
+int64_t gated_wgrad_workspace_bytes(int64_t hidden, int64_t nnz, int64_t tokens);
+cudaError_t launch_gated_wgrad(const void* x_planes, const void* d_planes, int64_t tokens, int64_t k, int64_t hidden, int64_t nnz,
+                               const void* plan, float* out, float* block_sumsq, void* workspace, cudaStream_t stream);
 
 struct AdapterCall {
     const void* x;           // [tokens, inner]

@@ -54,7 +54,7 @@ int bsmm_gated_act_backward(const void* pre, const void* dh, int64_t m, int64_t 
     if (too_large(m, 2 * hidden)) return BSMM_ERR_TOO_LARGE;
     return bsmm::report_cuda(bsmm::launch_gated_act_backward(
         pre, dh, m, hidden, dpre, dbias, static_cast<float*>(workspace), (flags & BSMM_GATED_GELU) != 0,
-        (flags & BSMM_GATED_PRE_BF16) != 0, (flags & BSMM_GATED_IO_BF16) != 0, static_cast<cudaStream_t>(stream)));
+        (flags & BSMM_GATED_PRE_BF16) != 0, (flags & BSMM_GATED_IO_BF16) != 0, nullptr, static_cast<cudaStream_t>(stream)));
 }
 
 int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, int64_t nnz,
@@ -89,28 +89,76 @@ int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t*
     return status != BSMM_OK ? status : bsmm_gated_act(pre, m, hidden, h, pass, stream);
 }
 
-// the bias gradient's partial sums and the weight gradient's: one after the other, in the same memory
+// Weight gradients of fp32 tensors in the fp32-class precisions come from planes of bf16 parts.
+static bool wgrad_from_planes(int64_t m, int64_t nnz, uint32_t precision) {
+    return m >= 64 && nnz > 0 && (precision == BSMM_PREC_TF32X3 || precision == BSMM_PREC_BF16X3);
+}
+static int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// [planes of x][planes of dpre][the bias gradient's partial sums and the weight gradient's: one after the other, in the same memory]
 int64_t bsmm_gated_backward_workspace_bytes(int64_t m, int64_t k, int64_t hidden, int64_t nnz, uint32_t flags) {
+    const uint32_t precision = flags & BSMM_PREC_MASK;
     const int64_t a = bsmm_gated_act_workspace_bytes(m, hidden);
-    const int64_t b = bsmm_sddmm_workspace_bytes(2 * hidden, k, m, nnz, flags & BSMM_PREC_MASK);
+    if (k < 0 || too_large(m, k) || nnz < 0 || nnz > 0x7fffffff) return -1;
+    if (a >= 0 && wgrad_from_planes(m, nnz, precision)) {
+        const int64_t b = bsmm::gated_wgrad_workspace_bytes(hidden, nnz, m);
+        return padded(6 * bsmm::plane_pitch(m) * k) + padded(12 * bsmm::plane_pitch(m) * hidden) + (a > b ? a : b);
+    }
+    const int64_t b = bsmm_sddmm_workspace_bytes(2 * hidden, k, m, nnz, precision);
     return a < 0 || b < 0 ? -1 : a > b ? a : b;
+}
+
+int64_t bsmm_gated_wgrad_plan_bytes(int64_t hidden, int64_t k, int64_t nnz) {
+    if (bsmm_gated_plan_bytes(hidden, k, nnz) < 0) return -1;
+    return bsmm::gated_wgrad_plan_bytes(hidden, nnz);
+}
+
+int bsmm_build_gated_wgrad_plan(const int32_t* ptr, const int32_t* idx, int64_t hidden, int64_t k, int64_t nnz, void* plan,
+                                bsmm_stream_t stream) {
+    (void)cudaGetLastError();
+    if (bsmm_gated_plan_bytes(hidden, k, nnz) < 0 || ptr == nullptr || plan == nullptr || (nnz > 0 && idx == nullptr) ||
+        !aligned(ptr, 4) || !aligned(idx, 8) || !aligned(plan, 16))
+        return BSMM_ERR_INVALID_ARGUMENT;
+    if (k > BSMM_GATED_MAX_K) return BSMM_ERR_TOO_LARGE;
+    return bsmm::report_cuda(bsmm::launch_build_gated_wgrad_plan(ptr, idx, hidden, k, nnz, plan, static_cast<cudaStream_t>(stream)));
 }
 
 int bsmm_gated_pass_backward(const void* x, const void* pre, const void* dh, int64_t m, int64_t k, const int32_t* idx,
                              const int32_t* csc_ptr, const int32_t* csc_idx, const int32_t* blocks, int64_t nnz,
                              const float* data, const void* packed, const void* csc_plan, const void* sddmm_plan,
-                             int64_t hidden, void* dpre, void* dx, float* dw, float* dbias, float* block_sumsq,
-                             void* workspace, uint32_t flags, bsmm_stream_t stream) {
+                             const void* wgrad_plan, int64_t hidden, void* dpre, void* dx, float* dw, float* dbias,
+                             float* block_sumsq, void* workspace, uint32_t flags, bsmm_stream_t stream) {
+    (void)cudaGetLastError();
     const uint32_t precision = flags & BSMM_PREC_MASK, pass = (flags >> 16) & 0xFu;
     if ((flags & ~(BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF) | BSMM_GATED_PASS(0xF))) != 0) return BSMM_ERR_UNSUPPORTED;
     // bf16 tensors: the products take them as they are, which the CUDA-core kernels of few tokens or no blocks do not
     const bool io16 = (pass & BSMM_GATED_IO_BF16) != 0;
     if (io16 && (precision != BSMM_PREC_BF16 || m < 32 || nnz == 0)) return BSMM_ERR_UNSUPPORTED;
-    int status = bsmm_gated_act_backward(pre, dh, m, hidden, dpre, dbias, workspace, pass, stream);
-    // the weight gradient first: in data-parallel training its all-reduce can overlap the input gradient
-    if (status == BSMM_OK && dw != nullptr)
-        status = bsmm_sddmm(dpre, x, 2 * hidden, k, m, dw, blocks, nnz, idx, sddmm_plan, block_sumsq, workspace,
-                            precision | (io16 ? BSMM_SDDMM_IO_BF16 : 0u), stream);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // the weight gradient before the input gradient: in data-parallel training its all-reduce can overlap the latter
+    int status = BSMM_OK;
+    if (dw != nullptr && wgrad_plan != nullptr && !io16 && wgrad_from_planes(m, nnz, precision)) {
+        if (m < 0 || hidden <= 0 || k <= 0 || (hidden % 32) != 0 || (k % 32) != 0 || x == nullptr || pre == nullptr || dh == nullptr ||
+            dpre == nullptr || workspace == nullptr || !aligned(x, 16) || !aligned(pre, 16) || !aligned(dh, 16) || !aligned(dpre, 16) ||
+            !aligned(dw, 16) || !aligned(dbias, 4) || !aligned(wgrad_plan, 16) || !aligned(workspace, 256))
+            return BSMM_ERR_INVALID_ARGUMENT;
+        if (gated_types(pass) != BSMM_OK || (pass & BSMM_GATED_X_BF16) != 0) return BSMM_ERR_UNSUPPORTED;
+        if (nnz > 0x7fffffff || k > BSMM_GATED_MAX_K || too_large(m, k) || too_large(m, 2 * hidden)) return BSMM_ERR_TOO_LARGE;
+        uint8_t* x_planes = static_cast<uint8_t*>(workspace);
+        uint8_t* d_planes = x_planes + padded(6 * bsmm::plane_pitch(m) * k);
+        uint8_t* rest = d_planes + padded(12 * bsmm::plane_pitch(m) * hidden);
+        cudaError_t err = bsmm::launch_gated_act_backward(pre, dh, m, hidden, dpre, dbias, reinterpret_cast<float*>(rest),
+                                                          (pass & BSMM_GATED_GELU) != 0, false, false, d_planes, s);
+        if (err == cudaSuccess) err = bsmm::launch_split_planes(static_cast<const float*>(x), m, k, x_planes, s);
+        if (err == cudaSuccess)
+            err = bsmm::launch_gated_wgrad(x_planes, d_planes, m, k, hidden, nnz, wgrad_plan, dw, block_sumsq, rest, s);
+        status = bsmm::report_cuda(err);
+    } else {
+        status = bsmm_gated_act_backward(pre, dh, m, hidden, dpre, dbias, workspace, pass, stream);
+        if (status == BSMM_OK && dw != nullptr)
+            status = bsmm_sddmm(dpre, x, 2 * hidden, k, m, dw, blocks, nnz, idx, sddmm_plan, block_sumsq, workspace,
+                                precision | (io16 ? BSMM_SDDMM_IO_BF16 : 0u), stream);
+    }
     if (status == BSMM_OK && dx != nullptr)
         status = bsmm_dsd(dpre, m, 2 * hidden, csc_ptr, csc_idx, nnz, data, packed, csc_plan, k, dx, nullptr,
                           (flags & (BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF))) | BSMM_DSD_DGRAD | (io16 ? BSMM_DSD_IO_BF16 : 0u), stream);

@@ -54,32 +54,50 @@ gated_act_kernel(const P* __restrict__ pre, int64_t quads, int64_t quads_per_row
 // dpre = [dh * u * act'(g) | dh * act(g)], column-interleaved like pre.  Memory bound: reads 3, writes 2 values per hidden
 // unit and token.  A CTA takes one block of 32 hidden units and kRowsPerChunk rows and also adds up its columns of dpre
 // (the bias gradient) in fp32, in a fixed order; sum_chunks_kernel adds the chunks in order, so results repeat bit by bit.
-template <typename P, typename H>
+// kPlanes: dpre also goes to its planes, the weight gradient's operand.
+template <typename P, typename H, bool kPlanes>
 __global__ void __launch_bounds__(256)
 gated_act_backward_kernel(const P* __restrict__ pre, const H* __restrict__ dh, int64_t m, int64_t hidden,
-                          H* __restrict__ dpre, float* __restrict__ partial, int act) {
+                          H* __restrict__ dpre, float* __restrict__ partial, int act,
+                          __nv_bfloat16* __restrict__ planes) {
     const int64_t blocks = hidden / 32;
     const int64_t chunk = blockIdx.x / blocks, block = blockIdx.x - chunk * blocks;
     const int lane8 = threadIdx.x & 7, row32 = threadIdx.x >> 3;
     const int64_t end = min(m, (chunk + 1) * kRowsPerChunk);
     float sum_g[4] = {0.f, 0.f, 0.f, 0.f}, sum_u[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t row = chunk * kRowsPerChunk + row32; row < end; row += 32) {
+    __shared__ float turned[kPlanes ? 64 : 1][33];  // 32 rows of the CTA's columns of dpre
+    for (int64_t row = chunk * kRowsPerChunk + row32; row - row32 < end; row += 32) {
         const int64_t at = row * 2 * hidden + block * 64 + lane8 * 4;
-        float g[4], u[4], d[4];
-        load4<P>(pre + at, g);
-        load4<P>(pre + at + 32, u);
-        load4<H>(dh + row * hidden + block * 32 + lane8 * 4, d);
+        float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+        if (row < end) {
+            float d[4];
+            load4<P>(pre + at, g);
+            load4<P>(pre + at + 32, u);
+            load4<H>(dh + row * hidden + block * 32 + lane8 * 4, d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float value, slope;
-            gate_act_grad(g[j], act, value, slope);
-            g[j] = d[j] * u[j] * slope;
-            u[j] = d[j] * value;
-            sum_g[j] += g[j];
-            sum_u[j] += u[j];
+            for (int j = 0; j < 4; ++j) {
+                float value, slope;
+                gate_act_grad(g[j], act, value, slope);
+                g[j] = d[j] * u[j] * slope;
+                u[j] = d[j] * value;
+                sum_g[j] += g[j];
+                sum_u[j] += u[j];
+            }
+            store4(dpre + at, g);
+            store4(dpre + at + 32, u);
         }
-        store4(dpre + at, g);
-        store4(dpre + at + 32, u);
+        if (kPlanes) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                turned[lane8 * 4 + j][row32] = g[j];
+                turned[32 + lane8 * 4 + j][row32] = u[j];
+            }
+            __syncthreads();
+            const int64_t pitch = plane_pitch(m), t = row - row32 + (threadIdx.x & 3) * 8, c = threadIdx.x >> 2;
+            if (t < pitch)
+                store_planes(turned[c] + (threadIdx.x & 3) * 8, planes + (block * 64 + c) * pitch + t, 2 * hidden * pitch);
+            __syncthreads();
+        }
     }
     if (partial == nullptr) return;
     __shared__ float sums[32][64];
@@ -117,23 +135,6 @@ constexpr int kSmallStages = 3;
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-
-// w = parts[0] + parts[1] + parts[2] exactly (3 x 8 significant bits), for a pair of values
-__device__ __forceinline__ void split3_bf16x2(float w0, float w1, uint32_t (&parts)[3]) {
-    asm("{\n\t.reg .b16 h0, h1, m1;\n\t.reg .f32 d0, d1;\n\t"
-        "mov.b16 m1, 0xBF80;\n\t"
-        "cvt.rn.bf16x2.f32 %0, %4, %3;\n\t"
-        "mov.b32 {h0, h1}, %0;\n\t"
-        "fma.rn.f32.bf16 d0, h0, m1, %3;\n\t"
-        "fma.rn.f32.bf16 d1, h1, m1, %4;\n\t"
-        "cvt.rn.bf16x2.f32 %1, d1, d0;\n\t"
-        "mov.b32 {h0, h1}, %1;\n\t"
-        "fma.rn.f32.bf16 d0, h0, m1, d0;\n\t"
-        "fma.rn.f32.bf16 d1, h1, m1, d1;\n\t"
-        "cvt.rn.bf16x2.f32 %2, d1, d0;\n\t}"
-        : "=&r"(parts[0]), "=&r"(parts[1]), "=r"(parts[2])
-        : "f"(w0), "f"(w1));
 }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -388,11 +389,12 @@ cudaError_t act_forward(const void* pre, int64_t m, int64_t hidden, void* h, int
     return cudaGetLastError();
 }
 
-template <typename P, typename H>
+template <typename P, typename H, bool kPlanes = false>
 cudaError_t act_backward(const void* pre, const void* dh, int64_t m, int64_t hidden, void* dpre, float* partial, int act,
-                         unsigned grid, cudaStream_t stream) {
-    gated_act_backward_kernel<P, H><<<grid, 256, 0, stream>>>(static_cast<const P*>(pre), static_cast<const H*>(dh), m, hidden,
-                                                              static_cast<H*>(dpre), partial, act);
+                         unsigned grid, cudaStream_t stream, void* planes = nullptr) {
+    gated_act_backward_kernel<P, H, kPlanes><<<grid, 256, 0, stream>>>(
+        static_cast<const P*>(pre), static_cast<const H*>(dh), m, hidden, static_cast<H*>(dpre), partial, act,
+        static_cast<__nv_bfloat16*>(planes));
     return cudaGetLastError();
 }
 
@@ -413,7 +415,7 @@ int64_t gated_act_workspace_bytes(int64_t m, int64_t hidden) { return row_chunks
 
 cudaError_t launch_gated_act_backward(const void* pre, const void* dh, int64_t m, int64_t hidden, void* dpre,
                                       float* dbias, float* workspace, int act, bool pre_bf16, bool io_bf16,
-                                      cudaStream_t stream) {
+                                      void* planes, cudaStream_t stream) {
     if (hidden == 0) return cudaSuccess;
     if (m > 0) {
         const int64_t ctas = row_chunks(m) * (hidden / 32);
@@ -421,7 +423,8 @@ cudaError_t launch_gated_act_backward(const void* pre, const void* dh, int64_t m
         float* partial = dbias != nullptr ? workspace : nullptr;
         const unsigned grid = (unsigned)ctas;
         const cudaError_t err =
-            !io_bf16 ? act_backward<float, float>(pre, dh, m, hidden, dpre, partial, act, grid, stream)
+            !io_bf16 && planes != nullptr ? act_backward<float, float, true>(pre, dh, m, hidden, dpre, partial, act, grid, stream, planes)
+            : !io_bf16 ? act_backward<float, float>(pre, dh, m, hidden, dpre, partial, act, grid, stream)
             : pre_bf16 ? act_backward<__nv_bfloat16, __nv_bfloat16>(pre, dh, m, hidden, dpre, partial, act, grid, stream)
                        : act_backward<float, __nv_bfloat16>(pre, dh, m, hidden, dpre, partial, act, grid, stream);
         if (err != cudaSuccess) return err;

@@ -827,9 +827,10 @@ void set_dsd_trace(long long* device_buffer, int block) {
     g_trace_block = block;
 }
 
-cudaError_t make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t elem_bytes, const void* base,
-                         uint64_t inner, uint64_t outer, uint32_t box_inner, uint32_t box_outer,
-                         CUtensorMapSwizzle swizzle) {
+namespace {
+// dims, box: innermost first; strides of the outer dimensions in bytes
+cudaError_t make_tmap(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint32_t rank, const cuuint64_t* dims,
+                      const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (fn == nullptr) return cudaErrorNotSupported;
     // The encoder is a driver entry point and wants a current context.  A thread that has made no runtime call
@@ -839,14 +840,30 @@ cudaError_t make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t e
     cudaError_t err = cudaGetDevice(&dev);
     if (err == cudaSuccess) err = cudaSetDevice(dev);
     if (err != cudaSuccess) return err;
-    const cuuint64_t dims[2] = {inner, outer};
-    const cuuint64_t strides[1] = {inner * elem_bytes};
-    const cuuint32_t box[2] = {box_inner, box_outer};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr,
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, dtype, rank, const_cast<void*>(base), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+}  // namespace
+
+cudaError_t make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t elem_bytes, const void* base,
+                         uint64_t inner, uint64_t outer, uint32_t box_inner, uint32_t box_outer,
+                         CUtensorMapSwizzle swizzle) {
+    const cuuint64_t dims[2] = {inner, outer};
+    const cuuint64_t strides[1] = {inner * elem_bytes};
+    const cuuint32_t box[2] = {box_inner, box_outer};
+    return make_tmap(map, dtype, base, 2, dims, strides, box, swizzle);
+}
+
+cudaError_t make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t elem_bytes, const void* base,
+                         uint64_t inner, uint64_t outer, uint64_t planes, uint64_t pitch, uint32_t box_inner,
+                         uint32_t box_outer, uint32_t box_planes, CUtensorMapSwizzle swizzle) {
+    const cuuint64_t dims[3] = {inner, outer, planes};
+    const cuuint64_t strides[2] = {pitch * elem_bytes, pitch * outer * elem_bytes};
+    const cuuint32_t box[3] = {box_inner, box_outer, box_planes};
+    return make_tmap(map, dtype, base, 3, dims, strides, box, swizzle);
 }
 
 cudaError_t device_status_address(unsigned int** addr) {

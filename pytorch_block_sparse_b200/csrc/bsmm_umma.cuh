@@ -98,6 +98,11 @@ cudaError_t make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t e
                          uint64_t inner, uint64_t outer, uint32_t box_inner, uint32_t box_outer,
                          CUtensorMapSwizzle swizzle);
 
+// 3-D tiled tensor map over a row-major [planes, outer, inner] array with rows of `pitch` elements.
+cudaError_t make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t elem_bytes, const void* base,
+                         uint64_t inner, uint64_t outer, uint64_t planes, uint64_t pitch, uint32_t box_inner,
+                         uint32_t box_outer, uint32_t box_planes, CUtensorMapSwizzle swizzle);
+
 // The sticky device status word of the current device: non-zero once a kernel gave up on a bounded
 // wait.  Kernels receive its address as a parameter.
 cudaError_t device_status_address(unsigned int** addr);

@@ -57,6 +57,8 @@ EXPORTS = (
     "bsmm_gated_pass_forward",
     "bsmm_gated_backward_workspace_bytes",
     "bsmm_gated_pass_backward",
+    "bsmm_gated_wgrad_plan_bytes",
+    "bsmm_build_gated_wgrad_plan",
     "bsmm_gated_plan_bytes",
     "bsmm_gated_images_bytes",
     "bsmm_build_gated_plan",
@@ -152,8 +154,12 @@ def load():
     lib.bsmm_gated_backward_workspace_bytes.restype = i64
     lib.bsmm_gated_backward_workspace_bytes.argtypes = [i64, i64, i64, i64, u32]
     lib.bsmm_gated_pass_backward.restype = i32
-    lib.bsmm_gated_pass_backward.argtypes = [vp, vp, vp, i64, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp,
-                                             vp, u32, vp]
+    lib.bsmm_gated_pass_backward.argtypes = [vp, vp, vp, i64, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp,
+                                             vp, vp, u32, vp]
+    lib.bsmm_gated_wgrad_plan_bytes.restype = i64
+    lib.bsmm_gated_wgrad_plan_bytes.argtypes = [i64, i64, i64]
+    lib.bsmm_build_gated_wgrad_plan.restype = i32
+    lib.bsmm_build_gated_wgrad_plan.argtypes = [vp, vp, i64, i64, i64, vp, vp]
     lib.bsmm_gated_plan_bytes.restype = i64
     lib.bsmm_gated_plan_bytes.argtypes = [i64, i64, i64]
     lib.bsmm_gated_images_bytes.restype = i64
@@ -662,6 +668,13 @@ class GatedPass:
         self.csr, self.csc = DsdPlan(ptr, idx), DsdPlan(csc_ptr, csc_idx)
         self.sddmm = SddmmPlan(ptr, idx)
         self.blocks = _aligned(blocks, 8)
+        lib, hidden, k = load(), self.csr.n_out_blocks * 16, self.csc.n_out_blocks * 32
+        self.wgrad = None
+        if k <= GATED_MAX_K:
+            self.wgrad = torch.empty(lib.bsmm_gated_wgrad_plan_bytes(hidden, k, self.csr.nnz), dtype=torch.uint8, device=ptr.device)
+            with _on(ptr.device):
+                check(lib.bsmm_build_gated_wgrad_plan(_ptr(self.csr.ptr), _ptr(self.csr.idx), hidden, k, self.csr.nnz,
+                                                      _ptr(self.wgrad), _stream(ptr.device)), "bsmm_build_gated_wgrad_plan")
 
     def forward(self, x, data, bias, activation, precision, out_dtype):
         """``(h, pre, packed)`` of a contiguous fp32 ``x``: ``pre`` fp32, ``packed`` the weight images (``None``: exact fp32)."""
@@ -712,7 +725,7 @@ class GatedPass:
                 lib.bsmm_gated_pass_backward(
                     x.data_ptr(), pre.data_ptr(), dh.data_ptr(), m, k, self.sddmm.idx.data_ptr(), csc.ptr.data_ptr(),
                     csc.idx.data_ptr(), self.blocks.data_ptr(), csc.nnz, data.data_ptr(), _ptr(packed), _ptr(plan),
-                    self.sddmm.buffer.data_ptr(), hidden, dpre.data_ptr(), _ptr(dx), _ptr(dw), _ptr(dbias), _ptr(sumsq),
+                    self.sddmm.buffer.data_ptr(), _ptr(self.wgrad), hidden, dpre.data_ptr(), _ptr(dx), _ptr(dw), _ptr(dbias), _ptr(sumsq),
                     ws.data_ptr(), flags, _stream(device)),
                 "bsmm_gated_pass_backward",
             )

@@ -8,6 +8,7 @@ import torch
 
 from pytorch_block_sparse_b200 import (AdapterRequests, BlockSparseGatedLinear, BlockSparseLinear, BlockSparseMatrix,
                                        LowRankAdapters, native)
+from pytorch_block_sparse_b200 import gated_linear
 from pytorch_block_sparse_b200.gated_linear import SMALL_TOKENS, interleave_rows, split_rows
 
 from .gpu_util import TOL, assert_device_healthy, randn
@@ -369,6 +370,33 @@ def test_the_bf16_kernel_alone(act, tokens, inner, hidden, density, same):
     assert rel(xg.grad, want[1]) <= bound("bf16", 4, torch.bfloat16, 1)
     assert rel(layer.weight.data.grad, in_data_layout(layer, want[2])) <= bound("bf16", 4, roundings=1)
     assert rel(layer.bias.grad, want[3]) <= bound("bf16", 4, roundings=1)
+    assert_device_healthy()
+
+
+@pytest.mark.parametrize("tokens,inner,hidden,density,same", [
+    (32, 32, 32, 1.0, True), (63, 64, 96, 1.0, True), (64, 32, 32, 1.0, True), (65, 64, 96, 1.0, True), (100, 544, 160, 0.5, False), (1024, 1056, 96, 0.4, True),
+    (1025, 96, 1184, 0.3, False), (2500, 2080, 64, 0.7, True), (6001, 256, 512, 0.2, True), (4096, 64, 4096, 0.6, False),
+])
+def test_the_fp32_weight_gradient(tokens, inner, hidden, density, same):
+    """Three bf16 parts of every value: what is dropped is 2^-24 of a term, the sums drift by 2e-8 per addition over segments
+    of 64: 2e-6 of the norm, far inside the 1e-5 of the precision's products."""
+    g = torch.Generator().manual_seed(tokens)
+    mask = torch.rand((hidden // 16, inner // 32), generator=g) < density
+    if same:
+        mask[1::2] = mask[0::2]
+    layer = make(inner, hidden, mask=mask, seed=tokens)
+    passes = gated_linear._gated_pass(layer.weight)
+    x, pre, dh = randn((tokens, inner), 1).cuda(), randn((tokens, 2 * hidden), 2).cuda(), randn((tokens, hidden), 3).cuda()
+    data = layer.weight.data.detach()
+    got = passes.backward(x, pre, dh, data, None, "silu", native.PREC_TF32X3, False, True, True)
+    dpre, _ = native.gated_act_backward(pre, dh, "silu", False)  # the product alone is on trial
+    want = in_data_layout(layer, dpre.cpu().double().t() @ x.cpu().double())
+    assert got[0] is None and torch.isfinite(got[1]).all()
+    assert rel(got[1], want) <= 2e-6
+    assert torch.allclose(got[3].cpu().double(), want.view(-1, 1024).square().sum(1), rtol=2e-5, atol=1e-12)
+    assert rel(got[2], dpre.cpu().double().sum(0)) <= 1e-6
+    again = passes.backward(x, pre, dh, data, None, "silu", native.PREC_TF32X3, False, True, True)
+    assert torch.equal(again[1], got[1]) and torch.equal(again[3], got[3])
     assert_device_healthy()
 
 
