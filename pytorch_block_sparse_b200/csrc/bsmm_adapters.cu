@@ -12,7 +12,8 @@
 //             each CTA writes an eighth of the outputs.  Inside a CTA the warps share the tile's distinct adapters and the
 //             features; fragments come straight from global memory
 //   tiles     (prompts) two launches: the shrink kernel writes v, the expand kernel multiplies by U_a.  A CTA owns 128 tokens
-//             of one request; the adapter's matrix passes through shared memory once for its eight warps
+//             of one request; the adapter's matrix passes through shared memory once for its eight warps.  (bf16 tensors,
+//             rank up to 128: the shrink kernel of bsmm_adapters_umma.cu)
 //
 // Arithmetic.  fp32 tensors: both operands are split into tf32 hi + lo parts and three products are added (about 2^-21
 // relative per term); bf16 tensors: x D is one exact product, v is split into bf16 hi + lo (its rounding to one bf16 would
@@ -20,16 +21,17 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
-#include "bsmm_feedforward.cuh"
+#include "bsmm_adapters.cuh"
 #include "bsmm_ptx.cuh"
 
 namespace bsmm {
 namespace {
 
+using namespace adapters;
+
 namespace cg = cooperative_groups;
 
 constexpr int kStep = 32;         // input features of one step
-constexpr int kNone = -1;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -155,12 +157,6 @@ __device__ __forceinline__ void load_pieces(Fragment<float, kLen>& f, const uint
         f.set(4 * i, v.x); f.set(4 * i + 1, v.y); f.set(4 * i + 2, v.z); f.set(4 * i + 3, v.w);
     }
 }
-
-// The expand kernel is launched while the shrink kernel still runs (programmatic dependent launch): what it does before
-// this wait -- finding its work, the first loads of U and of the base -- overlaps the other's tail.  Every thread waits before
-// it leaves, so that the expand grid never completes before the shrink grid.
-__device__ __forceinline__ void wait_for_shrink() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_expand_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ids[i] = adapter of token t0 + i, or kNone, for i < count <= 16; by one warp.  Offsets and ids come from the device
 // unchecked: whatever they hold, the search stays inside the arrays and ends, and an id outside [0, count) counts as none.
@@ -394,14 +390,8 @@ cluster_kernel(AdapterCall p, int tile_tokens, int64_t in_part, int64_t out_part
     cluster.barrier_wait();  // nobody leaves while its sums are read
 }
 
-struct Units {
-    int64_t tiles;      // of 128 tokens
-    int64_t parts;      // ranges of input features (shrink) or of output features (expand)
-    int64_t per_part;   // features of a part, a multiple of 32
-};
-
 // ---------------------------------------------------------------------------------------------- a CTA on 128 tokens
-constexpr int kTileTokens = 128, kTileWarps = 8, kTileThreads = 32 * kTileWarps;
+constexpr int kTileWarps = 8, kTileThreads = 32 * kTileWarps;
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -409,45 +399,6 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
-
-// Up to 128 tokens of one request.  The requests' tokens are cut into such tiles from each request's start; the tokens before
-// the first request and behind the last one count as requests without an adapter.
-struct Tile {
-    int first, rows, id;
-    // Each warp finds the tile by itself, 32 requests at a time.  False: there are fewer tiles.
-    __device__ __forceinline__ bool find(const AdapterCall& p, int tile) {
-        const int lane = threadIdx.x & 31, requests = (int)p.requests, tokens = (int)p.tokens;
-        int before = 0;
-        for (int r0 = -1; r0 <= requests; r0 += 32) {
-            const int r = r0 + lane;
-            int start = 0, end = 0, adapter = kNone;
-            if (r <= requests) {
-                start = r < 0 ? 0 : min(max(__ldg(p.offsets + r), 0), tokens);
-                end = r == requests ? tokens : min(max(__ldg(p.offsets + r + 1), 0), tokens);
-                if (r >= 0 && r < requests) adapter = __ldg(p.ids + r);
-                if (adapter < 0 || adapter >= p.count) adapter = kNone;
-            }
-            const int tiles = (max(end - start, 0) + kTileTokens - 1) / kTileTokens;
-            int sum = tiles;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int below = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += below;
-            }
-            const uint32_t reached = __ballot_sync(0xffffffffu, before + sum > tile);
-            if (reached != 0) {
-                const int src = __ffs(reached) - 1;
-                const int skipped = tile - before - __shfl_sync(0xffffffffu, sum - tiles, src);
-                first = __shfl_sync(0xffffffffu, start, src) + skipped * kTileTokens;
-                rows = min(kTileTokens, __shfl_sync(0xffffffffu, end, src) - first);
-                id = __shfl_sync(0xffffffffu, adapter, src);
-                return true;
-            }
-            before += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        return false;
-    }
-};
 
 // Shrink: a stage of the ring holds 128 bytes of k of the tile's tokens -- every lane copies the pieces that it will read
 // itself -- and of kRank rows of D, shared by the warps (16-byte piece c of row r at c ^ 4 (r mod 2): the two rows of a
@@ -596,25 +547,7 @@ expand_tile_kernel(AdapterCall p, Units units) {
     Tile tile;
     const bool found = tile.find(p, (int)(blockIdx.x % units.tiles));
     if (!found || tile.id == kNone) {
-        if (found && p.base != p.out) {  // tokens without an adapter keep their base: eight pieces in flight per thread
-            const int per_row = (int)(n1 - n0) / 8, pieces = tile.rows * per_row;
-            for (int i0 = threadIdx.x; i0 < pieces; i0 += 8 * kTileThreads) {
-                Raw8<O> v[8];
-                int64_t at[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int i = i0 + j * kTileThreads;
-                    at[j] = (tile.first + i / per_row) * p.outer + n0 + i % per_row * 8;
-                    if (i < pieces && p.base != nullptr) v[j].load(static_cast<const O*>(p.base) + at[j]);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (p.base != nullptr) v[j].unpack(f);
-                    if (i0 + j * kTileThreads < pieces) store8(static_cast<O*>(p.out) + at[j], f);
-                }
-            }
-        }
+        if (found) keep_base<O, kTileThreads>(p, tile, n0, n1);
         wait_for_shrink();
         return;
     }
@@ -742,69 +675,10 @@ expand_tile_kernel(AdapterCall p, Units units) {
     wait_copies<0>();
 }
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // Prompts go by tiles of 128 tokens, short requests and small batches by clusters.  us at 4096 -> 4096 features, rank 64,
 // clusters / tiles: 512 tokens in 2 requests 15 / 18, in 16 requests 15 / 19; 1024 tokens in 4 requests 29 / 20, in 32 29 / 28, in
 // 64 30 / 37; 4096 tokens in 64 requests 117 / 47, in 128 117 / 84, in 256 117 / 109 (rank 16: 66 / 29, 66 / 50, 66 / 71).
 bool by_tiles(int64_t tokens, int64_t requests) { return tokens >= 768 && tokens >= 32 * requests; }
-
-// How the input features are cut: CTAs of a cluster (a power of two up to 8), two per SM, at least 256 features each.  Tiles
-// start at each request's start, so that there may be one more for every request and for the tokens around them; half that is expected.
-Units tile_units(const AdapterCall& p) {
-    Units u;
-    u.tiles = ceil_div(p.tokens, kTileTokens) + p.requests + 2;
-    const int64_t expected = ceil_div(p.tokens, kTileTokens) + p.requests / 2;
-    u.parts = 1;
-    while (u.parts < 8 && expected * u.parts * 2 <= 2 * 148 && u.parts * 2 * 256 <= p.inner) u.parts *= 2;
-    u.per_part = ceil_div(ceil_div(p.inner, u.parts), 64) * 64;
-    return u;
-}
-
-// A launch in clusters of `cluster` CTAs, or one that may begin while the kernel before it still runs.
-template <typename... Params, typename... Args>
-cudaError_t launch_with(void (*kernel)(Params...), int64_t ctas, int threads, int smem, int cluster, bool early,
-                        cudaStream_t stream, Args... args) {
-    if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)ctas);
-    config.blockDim = dim3((unsigned)threads);
-    config.dynamicSmemBytes = (size_t)smem;
-    config.stream = stream;
-    cudaLaunchAttribute attr[1];
-    if (early) {
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-    } else {
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)cluster;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    }
-    config.attrs = attr;
-    config.numAttrs = early || cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
-template <typename Kernel>
-cudaError_t allow_smem(Kernel kernel, int bytes, bool (&ready)[64]) {  // per device; racing first calls set it twice
-    int dev = 0;
-    cudaError_t err = cudaGetDevice(&dev);
-    if (err != cudaSuccess) return err;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (ready[dev]) return cudaSuccess;
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (err == cudaSuccess) ready[dev] = true;
-    return err;
-}
-
-// the expand kernel's ranges of output features, in multiples of `unit`, for `wanted` CTAs or warps in all
-void cut_outputs(Units& u, int64_t outer, int64_t unit, int64_t wanted_parts) {
-    const int64_t most = ceil_div(outer, unit);
-    int64_t parts = wanted_parts < most ? wanted_parts : most;
-    parts = parts < 1 ? 1 : parts;
-    u.per_part = ceil_div(most, parts) * unit;
-    u.parts = ceil_div(outer, u.per_part);
-}
 
 template <typename T, typename O, int kRank>
 cudaError_t launch_tiles(const AdapterCall& p, cudaStream_t stream) {
@@ -813,12 +687,16 @@ cudaError_t launch_tiles(const AdapterCall& p, cudaStream_t stream) {
     cut_outputs(expand, p.outer, kExpandCols, 2 * 148 / (ceil_div(p.tokens, kTileTokens) + p.requests / 2));
     constexpr int kShrinkBytes = ShrinkTile<T, kRank>::kTotal;
     static bool shrink_ready[64] = {false}, expand_ready[64] = {false};
-    cudaError_t err = allow_smem(shrink_tile_kernel<T, kRank>, kShrinkBytes, shrink_ready);
-    if (err == cudaSuccess)
-        err = allow_smem(expand_tile_kernel<T, O, kRank>, ExpandTile<T, O, kRank>::total(kRank < 64 ? kRank : 256), expand_ready);
-    if (err == cudaSuccess)
-        err = launch_with(shrink_tile_kernel<T, kRank>, shrink.tiles * shrink.parts, kTileThreads, kShrinkBytes, (int)shrink.parts,
-                          false, stream, p, shrink);
+    cudaError_t err = allow_smem(expand_tile_kernel<T, O, kRank>, ExpandTile<T, O, kRank>::total(kRank < 64 ? kRank : 256), expand_ready);
+    if (err != cudaSuccess) return err;
+    if (shrink_on_umma(p, sizeof(T) == 2)) {
+        err = launch_shrink_umma(p, shrink, stream);
+    } else {
+        err = allow_smem(shrink_tile_kernel<T, kRank>, kShrinkBytes, shrink_ready);
+        if (err == cudaSuccess)
+            err = launch_with(shrink_tile_kernel<T, kRank>, shrink.tiles * shrink.parts, kTileThreads, kShrinkBytes, (int)shrink.parts,
+                              false, stream, p, shrink);
+    }
     if (err != cudaSuccess) return err;
     return launch_with(expand_tile_kernel<T, O, kRank>, expand.tiles * expand.parts, kTileThreads,
                        ExpandTile<T, O, kRank>::total(p.rank), 1, true, stream, p, expand);

@@ -6,7 +6,7 @@ import torch
 
 from pytorch_block_sparse_b200 import AdapterRequests, BlockSparseLinear, LowRankAdapters
 
-from .gpu_util import randn
+from .gpu_util import assert_device_healthy, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -95,6 +95,7 @@ def run_mix(lengths, ids, types, sizes):
         assert torch.equal(again, got)  # in place, and the same bits a second time
         alone = ad(x.cuda(), requests, dtype=out_dtype)
         check(alone, x, lengths, ids, weights, torch.zeros_like(base), dtype, inner, rank)
+    assert_device_healthy()
 
 
 PROMPTS = {  # long enough for the form that owns 128 tokens at a time
@@ -108,7 +109,8 @@ PROMPTS = {  # long enough for the form that owns 128 tokens at a time
 
 @pytest.mark.parametrize("mix", PROMPTS)
 @pytest.mark.parametrize("types", ["fp32", "bf16", "bf16 in fp32"])
-@pytest.mark.parametrize("sizes", [(32, 32, 1), (96, 160, 16), (1056, 544, 24), (544, 2080, 64), (64, 96, 200)])
+@pytest.mark.parametrize("sizes", [(32, 32, 1), (96, 160, 16), (1056, 544, 24), (544, 2080, 64), (64, 96, 200), (64, 64, 64),
+                                   (4128, 288, 48), (160, 4128, 128), (96, 32, 100)])
 def test_prompts(mix, types, sizes):
     run_mix(*PROMPTS[mix], types, sizes)
 
