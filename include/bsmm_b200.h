@@ -336,7 +336,8 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
  *   wgrad_plan                 bsmm_build_gated_wgrad_plan of the CSR, bsmm_gated_wgrad_plan_bytes bytes, 16-byte aligned, or NULL: with
  *                              it the weight gradient of fp32 tensors in BSMM_PREC_TF32X3 and BSMM_PREC_BF16X3 (64 tokens or more)
  *                              comes from a kernel that multiplies three bf16 parts of every value and shares the input
- *                              between gate and up blocks (relative error near 1e-6), else from bsmm_sddmm
+ *                              between gate and up blocks (relative error near 1e-6; magnitudes above bf16's largest finite value,
+ *                              3.39e38, round to infinity), else from bsmm_sddmm
  *   workspace                  bsmm_gated_backward_workspace_bytes bytes, 256-byte aligned
  */
 #define BSMM_GATED_PASS(f) (((uint32_t)(f)&0xFu) << 16)

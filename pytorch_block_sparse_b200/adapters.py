@@ -104,8 +104,10 @@ class LowRankAdapters(nn.Module):
         lead, kind = x.shape[:-1], x.dtype
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise Exception("Invalid input %s for adapters of %d features" % (tuple(x.shape), self.in_features))
-        if kind is not down.dtype:
-            raise ValueError("x is %s, the adapters are %s" % (kind, down.dtype))
+        if kind is not down.dtype or kind is not up.dtype or (kind is not torch.float32 and kind is not torch.bfloat16):
+            raise ValueError("x is %s, the adapters are %s: expected one type, float32 or bfloat16" % (kind, down.dtype))
+        if scaling.dtype is not torch.float32:  # (the module was cast as a whole)
+            scaling = scaling.float()
         device = down.device
         if x.device != device or requests.offsets.device != device or (base is not None and base.device != device):
             raise native.NativeError("x, the requests, the base and the adapters must be on one device, got %s, %s, %s, %s" % (

@@ -16,7 +16,10 @@ from torch.autograd.function import once_differentiable
 from . import native
 from .block_sparse import BlockSparseMatrix
 
-# Up to this many tokens inference computes from the stored blocks directly (``bsmm_gated_small``).
+# Up to this many tokens inference computes from the stored blocks directly (``bsmm_gated_small``).  us, few-token kernel / weight
+# images and tensor-core kernel, on one B200: bf16, 4096 -> 8192 at density 0.25, 16 tokens 21 / 44, 32 tokens 26 / 44, 48 tokens
+# 42 / 44, 64 tokens 44 / 44; 4096 -> 16384 at 0.1, 32 tokens 29 / 32, 48 tokens 46 / 32; 1024 -> 2048 at 0.5, 32 tokens 12 / 15.
+# fp32, 4096 -> 8192: 16 tokens 40 / 98, 32 tokens 69 / 98, 48 tokens 99 / 98.
 SMALL_TOKENS = 32
 
 
@@ -195,6 +198,10 @@ class BlockSparseGatedLinear(nn.Module):
             raise ValueError("BlockSparseGatedLinear takes float32 or bfloat16 tensors, got %s" % x.dtype)
         if not data.is_cuda:
             weight._require_cuda()
+        if data.dtype is not torch.float32:
+            raise Exception("BlockSparseGatedLinear weights should be float32, not of type %s" % data.dtype)
+        if bias is not None and bias.dtype is not torch.float32:
+            bias = bias.float()
         if x.device != data.device:
             raise native.NativeError("x is on %s, the layer on %s" % (x.device, data.device))
         flat = (x if len(shape) == 2 else x.reshape(-1, shape[-1])).contiguous()

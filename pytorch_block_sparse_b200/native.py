@@ -675,6 +675,19 @@ class GatedPass:
             with _on(ptr.device):
                 check(lib.bsmm_build_gated_wgrad_plan(_ptr(self.csr.ptr), _ptr(self.csr.idx), hidden, k, self.csr.nnz,
                                                       _ptr(self.wgrad), _stream(ptr.device)), "bsmm_build_gated_wgrad_plan")
+        self.built, self.groups = _Built(), set()
+        with _on(ptr.device):
+            self.built.mark(ptr.device)
+
+    def _buffer(self, plan, m, precision, device):
+        """``(group, plan buffer)`` of one of the two products, built on first use."""
+        group = plan.group_for(m, precision)
+        buffer = plan.buffer(group)
+        if (plan is self.csr, group) not in self.groups and not capturing():
+            with _on(device):
+                self.built.mark(device)
+            self.groups.add((plan is self.csr, group))
+        return group, buffer
 
     def forward(self, x, data, bias, activation, precision, out_dtype):
         """``(h, pre, packed)`` of a contiguous fp32 ``x``: ``pre`` fp32, ``packed`` the weight images (``None``: exact fp32)."""
@@ -687,12 +700,12 @@ class GatedPass:
         flags = precision | (_gated_flags(activation) | (GATED_IO_BF16 if out_dtype is torch.bfloat16 else 0)) << 16
         plan = packed = None
         if precision != PREC_FP32_SIMT:
-            group = csr.group_for(m, precision)
-            plan = csr.buffer(group)
+            group, plan = self._buffer(csr, m, precision, device)
             flags |= group << 8
             packed = torch.empty(max(16, lib.bsmm_packed_bytes(csr.nnz, precision)), dtype=torch.uint8, device=device)
         x, data, bias = _aligned(x), _aligned(data), _aligned(bias)
         with _on(device):
+            self.built.join(_stream(device), device, (plan,))
             check(
                 lib.bsmm_gated_pass_forward(
                     x.data_ptr(), m, k, csr.ptr.data_ptr(), csr.idx.data_ptr(), csr.nnz, data.data_ptr(), _ptr(packed), _ptr(plan),
@@ -716,11 +729,11 @@ class GatedPass:
         ws = torch.empty(max(16, lib.bsmm_gated_backward_workspace_bytes(m, k, hidden, csc.nnz, flags)), dtype=torch.uint8, device=device)
         plan = None
         if precision != PREC_FP32_SIMT and want_x:
-            group = csc.group_for(m, precision)
-            plan = csc.buffer(group)
+            group, plan = self._buffer(csc, m, precision, device)
             flags |= group << 8
         x, dh, data = _aligned(x), _aligned(dh), _aligned(data)
         with _on(device):
+            self.built.join(_stream(device), device, (plan, self.wgrad, self.sddmm.buffer))
             check(
                 lib.bsmm_gated_pass_backward(
                     x.data_ptr(), pre.data_ptr(), dh.data_ptr(), m, k, self.sddmm.idx.data_ptr(), csc.ptr.data_ptr(),
@@ -754,6 +767,30 @@ def gated_small(x, ptr, idx, data, hidden, bias, activation, out_dtype):
 GATED_MAX_K = 131072
 
 
+class _Built:
+    """When and where plans were built, so that work on another stream waits for them."""
+
+    def __init__(self):
+        self.stream = self.event = None
+
+    def mark(self, device):
+        """Plans were built on ``device``'s current stream just now.  (While capturing they belong to the graph alone.)"""
+        self.stream = _stream(device)
+        self.event = None if capturing() else torch.cuda.current_stream(device).record_event()
+
+    def join(self, stream, device, buffers):
+        """Work on ``stream`` may read ``buffers`` from here on.  Nothing is asked while capturing, where an event from outside may
+        not be: a capture begins with an idle device."""
+        if stream == self.stream or self.event is None or capturing():
+            return
+        current = torch.cuda.current_stream(device)
+        if not self.event.query():
+            current.wait_event(self.event)
+        for t in buffers:
+            if t is not None:
+                t.record_stream(current)
+
+
 class GatedPlan:
     """Launch plan of the gated block's tensor-core kernel for one (offsets, indices) pair of the interleaved matrix."""
 
@@ -763,21 +800,11 @@ class GatedPlan:
         self.ptr, self.idx = ptr, idx = _aligned(ptr, 4), _aligned(idx, 8)
         self.hidden, self.k, self.nnz = hidden, k, idx.shape[0]
         self.buffer = torch.empty(lib.bsmm_gated_plan_bytes(hidden, k, self.nnz), dtype=torch.uint8, device=ptr.device)
+        self.built = _Built()
         with _on(ptr.device):
-            self.stream = _stream(ptr.device)
-            check(lib.bsmm_build_gated_plan(_ptr(ptr), _ptr(idx), hidden, k, self.nnz, _ptr(self.buffer), self.stream),
+            check(lib.bsmm_build_gated_plan(_ptr(ptr), _ptr(idx), hidden, k, self.nnz, _ptr(self.buffer), _stream(ptr.device)),
                   "bsmm_build_gated_plan")
-            self.event = None if capturing() else torch.cuda.current_stream(ptr.device).record_event()
-
-    def on(self, stream):
-        """The plan's address for work on ``stream``: another stream than the one that built it waits for the build.  (Not
-        while capturing, where an event from outside may not be asked: a capture begins with an idle device.)"""
-        if stream != self.stream and self.event is not None and not capturing():
-            current = torch.cuda.current_stream(self.buffer.device)
-            if not self.event.query():
-                current.wait_event(self.event)
-            self.buffer.record_stream(current)
-        return self.buffer.data_ptr()
+            self.built.mark(ptr.device)
 
 
 def gated_forward(x, plan, data, bias, activation, keep_pre):
@@ -793,7 +820,8 @@ def gated_forward(x, plan, data, bias, activation, keep_pre):
     flags = _gated_flags(activation) | GATED_IO_BF16 | GATED_PRE_BF16
     with _on(x.device):
         stream = _stream(x.device)
-        at = plan.on(stream)
+        plan.built.join(stream, x.device, (plan.buffer,))
+        at = plan.buffer.data_ptr()
         check(lib.bsmm_gated_pack(_ptr(data), at, plan.hidden, plan.k, plan.nnz, _ptr(images), stream),
               "bsmm_gated_pack")
         check(
