@@ -144,6 +144,19 @@ cudaError_t launch_pack_pairs(const float* data, const void* plan, int64_t hidde
 cudaError_t launch_gated_umma(const void* x, int64_t m, int64_t k, const void* plan, const void* images, int64_t hidden,
                               const float* bias, void* h, void* pre, int act, cudaStream_t stream);
 
+// the forward pass of fp32 tensors from planes of three bf16 parts (bsmm_gated_f32.cu)
+int64_t gated_f32_workspace_bytes(int64_t m, int64_t k, int64_t nnz);
+cudaError_t launch_gated_f32(const float* x, int64_t m, int64_t k, const float* data, int64_t nnz, const int32_t* ptr,
+                             const void* pairs_plan, int64_t hidden, const float* bias, float* h, float* pre, int act, void* workspace,
+                             cudaStream_t stream);
+
+// The rows' pairs in the plan of bsmm_build_gated_wgrad_plan: a row's begin where its entries do in the CSR.
+struct GatedPairs {
+    const int4* pairs;       // (input block, gate slot, up slot, 0), a slot -1 where that projection has no block
+    const int32_t* counts;   // per pair-row
+};
+GatedPairs gated_pairs(const void* plan, int64_t hidden, int64_t nnz);
+
 // the weight gradient of fp32 tensors from planes of three bf16 parts (bsmm_gated_wgrad.cu)
 int64_t gated_wgrad_plan_bytes(int64_t hidden, int64_t nnz);
 cudaError_t launch_build_gated_wgrad_plan(const int32_t* ptr, const int32_t* idx, int64_t hidden, int64_t k, int64_t nnz, void* plan,

@@ -74,26 +74,45 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
                                                       static_cast<cudaStream_t>(stream)));
 }
 
+// The fp32-class precisions multiply planes of bf16 parts.
+static bool from_planes(int64_t nnz, uint32_t precision) {
+    return nnz > 0 && (precision == BSMM_PREC_TF32X3 || precision == BSMM_PREC_BF16X3);
+}
+static bool wgrad_from_planes(int64_t m, int64_t nnz, uint32_t precision) { return m >= 64 && from_planes(nnz, precision); }
+static int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+int64_t bsmm_gated_forward_workspace_bytes(int64_t m, int64_t k, int64_t hidden, int64_t nnz, uint32_t flags) {
+    if (m < 0 || k < 0 || hidden < 0 || nnz < 0 || nnz > 0x7fffffff || too_large(m, k)) return -1;
+    return from_planes(nnz, flags & BSMM_PREC_MASK) ? bsmm::gated_f32_workspace_bytes(m, k, nnz) : 0;
+}
+
 int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, int64_t nnz,
-                            const float* data, void* packed, const void* plan, int64_t hidden, const float* bias, float* pre,
-                            void* h, uint32_t flags, bsmm_stream_t stream) {
+                            const float* data, void* packed, const void* plan, const void* wgrad_plan, int64_t hidden,
+                            const float* bias, float* pre, void* h, void* workspace, uint32_t flags, bsmm_stream_t stream) {
+    (void)cudaGetLastError();
     const uint32_t precision = flags & BSMM_PREC_MASK, pass = (flags >> 16) & 0xFu;
     if ((flags & ~(BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF) | BSMM_GATED_PASS(0xF))) != 0 || (pass & BSMM_GATED_PRE_BF16) != 0)
         return BSMM_ERR_UNSUPPORTED;
-    if (precision != BSMM_PREC_FP32_SIMT) {
+    if (precision != BSMM_PREC_FP32_SIMT && packed != nullptr) {
         const int status = bsmm_pack_weights(data, nnz, precision, packed, nullptr, stream);
         if (status != BSMM_OK) return status;
     }
+    if (wgrad_plan != nullptr && pass == (pass & BSMM_GATED_GELU) && from_planes(nnz, precision)) {
+        if (m < 0 || k <= 0 || hidden < 0 || (hidden % 32) != 0 || (k % 32) != 0) return BSMM_ERR_INVALID_ARGUMENT;
+        if (m == 0 || hidden == 0) return BSMM_OK;
+        if (x == nullptr || ptr == nullptr || data == nullptr || h == nullptr || workspace == nullptr) return BSMM_ERR_INVALID_ARGUMENT;
+        if (!aligned(x, 16) || !aligned(ptr, 4) || !aligned(data, 16) || !aligned(wgrad_plan, 16) || !aligned(bias, 16) ||
+            !aligned(pre, 16) || !aligned(h, 16) || !aligned(workspace, 256))
+            return BSMM_ERR_INVALID_ARGUMENT;
+        if (nnz > 0x7fffffff || k > BSMM_GATED_MAX_K || too_large(m, k) || too_large(m, 2 * hidden)) return BSMM_ERR_TOO_LARGE;
+        return bsmm::report_cuda(bsmm::launch_gated_f32(x, m, k, data, nnz, ptr, wgrad_plan, hidden, bias, static_cast<float*>(h), pre,
+                                                        (pass & BSMM_GATED_GELU) != 0, workspace, static_cast<cudaStream_t>(stream)));
+    }
+    if (pre == nullptr && m > 0 && hidden > 0) return BSMM_ERR_INVALID_ARGUMENT;
     const int status = bsmm_dsd(x, m, k, ptr, idx, nnz, data, packed, plan, 2 * hidden, pre, bias,
                                 flags & (BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF)), stream);
     return status != BSMM_OK ? status : bsmm_gated_act(pre, m, hidden, h, pass, stream);
 }
-
-// Weight gradients of fp32 tensors in the fp32-class precisions come from planes of bf16 parts.
-static bool wgrad_from_planes(int64_t m, int64_t nnz, uint32_t precision) {
-    return m >= 64 && nnz > 0 && (precision == BSMM_PREC_TF32X3 || precision == BSMM_PREC_BF16X3);
-}
-static int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // [planes of x][planes of dpre][the bias gradient's partial sums and the weight gradient's: one after the other, in the same memory]
 int64_t bsmm_gated_backward_workspace_bytes(int64_t m, int64_t k, int64_t hidden, int64_t nnz, uint32_t flags) {

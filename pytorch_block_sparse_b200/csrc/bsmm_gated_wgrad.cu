@@ -359,6 +359,11 @@ void choose_splits(int64_t rows, int64_t nnz, int64_t tokens, int64_t* splits, i
 
 }  // namespace
 
+GatedPairs gated_pairs(const void* plan, int64_t hidden, int64_t nnz) {
+    const PlanPointers at = plan_pointers(const_cast<void*>(plan), hidden, nnz);
+    return {at.pairs, at.counts};
+}
+
 int64_t gated_wgrad_plan_bytes(int64_t hidden, int64_t nnz) {
     return 16 + 16 * max_items(hidden / 32, nnz) + 16 * nnz + (hidden / 32 + 1) * 4;
 }

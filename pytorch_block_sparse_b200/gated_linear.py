@@ -219,7 +219,7 @@ class BlockSparseGatedLinear(nn.Module):
         if _fused(flat, prec):
             return native.gated_forward(flat, _gated_plan(weight), data, bias, self.activation, False)[0]
         x = flat if flat.dtype is torch.float32 else flat.float()
-        return _gated_pass(weight).forward(x, data, bias, self.activation, prec, _out_dtype(flat, prec))[0]
+        return _gated_pass(weight).forward(x, data, bias, self.activation, prec, _out_dtype(flat, prec), keep=False)[0]
 
     def extra_repr(self):
         return "in_features={}, hidden_features={}, bias={}, activation={}, block_count={}".format(

@@ -55,6 +55,7 @@ EXPORTS = (
     "bsmm_gated_act_backward",
     "bsmm_gated_small",
     "bsmm_gated_pass_forward",
+    "bsmm_gated_forward_workspace_bytes",
     "bsmm_gated_backward_workspace_bytes",
     "bsmm_gated_pass_backward",
     "bsmm_gated_wgrad_plan_bytes",
@@ -150,7 +151,9 @@ def load():
     lib.bsmm_gated_small.restype = i32
     lib.bsmm_gated_small.argtypes = [vp, i64, i64, vp, vp, i64, vp, i64, vp, vp, u32, vp]
     lib.bsmm_gated_pass_forward.restype = i32
-    lib.bsmm_gated_pass_forward.argtypes = [vp, i64, i64, vp, vp, i64, vp, vp, vp, i64, vp, vp, vp, u32, vp]
+    lib.bsmm_gated_pass_forward.argtypes = [vp, i64, i64, vp, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, u32, vp]
+    lib.bsmm_gated_forward_workspace_bytes.restype = i64
+    lib.bsmm_gated_forward_workspace_bytes.argtypes = [i64, i64, i64, i64, u32]
     lib.bsmm_gated_backward_workspace_bytes.restype = i64
     lib.bsmm_gated_backward_workspace_bytes.argtypes = [i64, i64, i64, i64, u32]
     lib.bsmm_gated_pass_backward.restype = i32
@@ -689,27 +692,33 @@ class GatedPass:
             self.groups.add((plan is self.csr, group))
         return group, buffer
 
-    def forward(self, x, data, bias, activation, precision, out_dtype):
-        """``(h, pre, packed)`` of a contiguous fp32 ``x``: ``pre`` fp32, ``packed`` the weight images (``None``: exact fp32)."""
+    def forward(self, x, data, bias, activation, precision, out_dtype, keep=True):
+        """``(h, pre, packed)`` of a contiguous fp32 ``x``: for backward (``keep``) ``pre`` in fp32 and the weight images (``None`` for
+        exact fp32)."""
         _need_cuda(x, "x")
         lib, csr, device = load(), self.csr, x.device
         m, k = x.shape
         hidden = csr.n_out_blocks * 16
-        pre = torch.empty((m, 2 * hidden), dtype=torch.float32, device=device)
-        h = torch.empty((m, hidden), dtype=out_dtype, device=device)
         flags = precision | (_gated_flags(activation) | (GATED_IO_BF16 if out_dtype is torch.bfloat16 else 0)) << 16
-        plan = packed = None
-        if precision != PREC_FP32_SIMT:
+        ws_bytes = lib.bsmm_gated_forward_workspace_bytes(m, k, hidden, csr.nnz, flags) if self.wgrad is not None else 0
+        whole = ws_bytes > 0  # one kernel for projections, activation and product
+        h = torch.empty((m, hidden), dtype=out_dtype, device=device)
+        pre = torch.empty((m, 2 * hidden), dtype=torch.float32, device=device) if keep or not whole else None
+        plan = packed = ws = None
+        if whole:
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+        elif precision != PREC_FP32_SIMT:
             group, plan = self._buffer(csr, m, precision, device)
             flags |= group << 8
+        if precision != PREC_FP32_SIMT and (keep or not whole):
             packed = torch.empty(max(16, lib.bsmm_packed_bytes(csr.nnz, precision)), dtype=torch.uint8, device=device)
         x, data, bias = _aligned(x), _aligned(data), _aligned(bias)
         with _on(device):
-            self.built.join(_stream(device), device, (plan,))
+            self.built.join(_stream(device), device, (plan, self.wgrad))
             check(
                 lib.bsmm_gated_pass_forward(
                     x.data_ptr(), m, k, csr.ptr.data_ptr(), csr.idx.data_ptr(), csr.nnz, data.data_ptr(), _ptr(packed), _ptr(plan),
-                    hidden, _ptr(bias), pre.data_ptr(), h.data_ptr(), flags, _stream(device)),
+                    _ptr(self.wgrad) if whole else None, hidden, _ptr(bias), _ptr(pre), h.data_ptr(), _ptr(ws), flags, _stream(device)),
                 "bsmm_gated_pass_forward",
             )
         return h, pre, packed

@@ -59,8 +59,15 @@ def test_gated_kernel_entry_points():
     assert run(null, 0, 32, null, null, 0, 32, null, null, null, both, null) == OK
     assert lib.bsmm_build_gated_wgrad_plan(fake, fake, 32, 48, 1, fake, null) == INVALID
     passes = lib.bsmm_gated_pass_forward
-    assert passes(fake, 4, 32, fake, fake, 1, fake, null, null, 32, null, fake, fake, 1 << 30, null) == UNSUPPORTED
-    assert passes(fake, 4, 48, fake, fake, 1, fake, null, null, 32, null, fake, fake, 0, null) == INVALID
+    x3 = native.PREC_TF32X3
+    assert passes(fake, 4, 32, fake, fake, 1, fake, null, null, null, 32, null, fake, fake, null, 1 << 30, null) == UNSUPPORTED
+    assert passes(fake, 4, 48, fake, fake, 1, fake, null, null, null, 32, null, fake, fake, null, 0, null) == INVALID
+    assert passes(fake, 4, 32, fake, fake, 1, fake, null, null, null, 32, null, null, fake, null, 0, null) == INVALID  # no pre
+    assert passes(fake, 4, 32, fake, fake, 1, fake, null, null, fake, 32, null, null, fake, null, x3, null) == INVALID  # no workspace
+    assert passes(fake, 4, 32, fake, fake, 1, fake, null, null, fake, 32, odd, null, fake, fake, x3, null) == INVALID
+    assert passes(fake, 4, native.GATED_MAX_K + 32, fake, fake, 1, fake, null, null, fake, 32, null, null, fake, fake, x3, null) == TOO_LARGE
+    assert lib.bsmm_gated_forward_workspace_bytes(-1, 32, 32, 1, x3) == -1
+    assert lib.bsmm_gated_forward_workspace_bytes(4, 32, 32, 1, 0) == 0
     back = lib.bsmm_gated_pass_backward
     args = [fake, fake, fake, 64, 32, fake, fake, fake, fake, 1, fake, fake, fake, fake, fake, 32, fake, null, fake, null, null, fake]
     assert back(*args[:-1], null, native.PREC_TF32X3, null) == INVALID                     # no workspace

@@ -400,6 +400,34 @@ def test_the_fp32_weight_gradient(tokens, inner, hidden, density, same):
     assert_device_healthy()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("tokens,inner,hidden,density,same", [
+    (1, 32, 32, 1.0, True), (33, 64, 96, 1.0, True), (128, 544, 160, 0.5, False), (129, 1056, 96, 0.4, True),
+    (256, 96, 1184, 0.3, False), (257, 2080, 64, 0.7, True), (1000, 4096, 96, 0.9, True), (700, 64, 4096, 0.6, False),
+])
+def test_the_fp32_kernel_alone(act, tokens, inner, hidden, density, same):
+    """g and u to 2e-6 of their norm (three bf16 parts: 2^-24 of a term is dropped; the sums drift by 2e-8 per addition over
+    segments of 64), rows longer than a segment among them; h by 3 times that, the same with and without g and u kept."""
+    g = torch.Generator().manual_seed(tokens)
+    mask = torch.rand((hidden // 16, inner // 32), generator=g) < density
+    if same:
+        mask[1::2] = mask[0::2]
+    mask[:2] = True
+    layer = make(inner, hidden, act=act, mask=mask, seed=tokens)
+    x = randn((tokens, inner), 1)
+    passes = gated_linear._gated_pass(layer.weight)
+    data, bias = layer.weight.data.detach(), layer.bias.detach()
+    h, pre, packed = passes.forward(x.cuda(), data, bias, act, native.PREC_TF32X3, torch.float32)
+    assert packed is not None and torch.isfinite(pre).all()
+    want = x.double() @ layer.weight.to_dense().detach().cpu().double().t() + bias.cpu().double()
+    assert rel(pre, want) <= 2e-6
+    assert rel(h, reference(layer, x)) <= 6e-6
+    alone = passes.forward(x.cuda(), data, bias, act, native.PREC_TF32X3, torch.float32, keep=False)
+    assert alone[1] is None and alone[2] is None and torch.equal(alone[0], h)
+    assert torch.equal(native.gated_act(pre, act, torch.float32), h)
+    assert_device_healthy()
+
+
 def test_from_linears_and_state_dict():
     torch.manual_seed(0)
     gate, up = torch.nn.Linear(96, 64), torch.nn.Linear(96, 64)
