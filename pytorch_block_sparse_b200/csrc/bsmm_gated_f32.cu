@@ -12,8 +12,9 @@
 // pair: 48 KiB of x (three TMA boxes, 64-byte swizzle) and its image, 12 instructions, ~840 cycles at the nominal rate; with 128
 // tokens per tile it moves 36 KiB for half of that and is bound by L2 -> shared memory.  Persistent, one CTA per SM:
 //   warp 0 loads, warp 1 issues, warps 2-9 read out (four per half), the sums and h through shared memory in whole lines.
-// Bound by the tensor cores.  8192 tokens, 4096 -> 2 x 4096 at density 0.25 with g and u kept: 713 us, 1160 TFLOP/s (759 with each lane storing
-// its own token) + 52 to split x + 19 for the images; bsmm_dsd in TF32x3 and bsmm_gated_act as kernels of their own take 941.
+// Bound by the tensor cores.  8192 tokens, 4096 -> 2 x 4096 at density 0.25 with g and u kept: 720 us, 1145 TFLOP/s (713 with
+// segments of 32 pairs, but a relative error of 1.8e-6 instead of 0.9e-6; 759 with each lane storing its own token) + 52 to split
+// x + 19 for the images; bsmm_dsd in TF32x3 and bsmm_gated_act as kernels of their own take 941.
 // Without g and u kept, TF32x3 products before -> this kernel, us (device, images and split included):
 //   4096 tokens, 1024 -> 2 x 4096 at 0.5: 230 -> 185   512: 70 -> 41   64: 39 -> 23
 //   4096 tokens, 8192 -> 2 x 2048 at 0.25: 414 -> 400  512: 93 -> 81   64: 91 -> 53
@@ -33,7 +34,7 @@ namespace {
 using namespace ptx;
 
 constexpr int kHalves = 2, kTileTokens = 128 * kHalves, kPlanes = 3;
-constexpr int kSegment = 32;
+constexpr int kSegment = 16;
 constexpr uint32_t kPlaneBytes = kTileTokens * 64;     // [256 tokens][32 k] bf16
 constexpr uint32_t kXBytes = kPlanes * kPlaneBytes;
 constexpr uint32_t kImageBytes = 192 * 32 * 2;         // [g1 u1 g2 u2 g3 u3][32 k] bf16

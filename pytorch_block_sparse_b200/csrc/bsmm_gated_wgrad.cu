@@ -7,8 +7,8 @@
 // tokens compute them for both projections at once, each into the columns of its order of magnitude:
 //   x1 * [d1 d2 d3] (N = 192)    x2 * [d1 d2] (N = 128, 64 columns further)    x3 * [d1] (N = 64, 128 further)
 // so that column set k holds the terms of order 2^-8k and the sets are added once, at the end of a segment of tokens.  The tensor
-// core's own accumulation drifts by about 2e-8 per addition; segments of 1024 tokens (64 additions) keep that near 1e-6, their
-// sums are added in fp32 registers.
+// core's own accumulation drifts by about 2e-8 per addition; segments of 512 tokens (32 additions) keep that near 5e-7, their
+// sums are added in fp32 registers (segments of 1024: 757 us instead of 772 on the case below, error 1.6e-6 instead of 1.05e-6).
 //
 // The three parts are written beforehand as three bf16 matrices ("planes"), transposed: [features][tokens], for x by
 // split_planes_kernel and for [dg | du] by the activation's backward kernel: tokens are the contraction index, and rows of
@@ -16,8 +16,8 @@
 //
 // CTA = one item (up to 4 pairs of one pair-row, which fill the 128 rows of an instruction) x one range of tokens.  Per 64 tokens:
 // 48 KiB of x, 24 KiB of [dg | du], 12 instructions.  Bound by the tensor core: 8192 tokens, 4096 -> 4096 at density 0.25 take
-// 774 us, 1080 TFLOP/s of the six products together where a large dense bf16 product reaches 1390 under the power limit
-// (without the loads 679 us, without the instructions 543).  bsmm_sddmm takes 1230 us on the same operands.  Token-major
+// 772 us, 1070 TFLOP/s of the six products together where a large dense bf16 product reaches 1390 under the power limit
+// (segments of 1024 tokens: 774 us at that time, without the loads 679, without the instructions 543).  bsmm_sddmm takes 1230 us on the same operands.  Token-major
 // planes (MN-major operands, 8 pairs per item) measured the same.
 //   warp 0 loads, warp 1 issues, warps 2-5 read the sums out.
 // Token ranges write partial results that reduce_kernel adds in order; every result repeats bit by bit.
@@ -35,7 +35,7 @@ using namespace ptx;
 
 constexpr int kItemPairs = 4;
 constexpr int kStepTokens = 64;
-constexpr int kSegmentSteps = 16;                              // 1024 tokens between two promotions
+constexpr int kSegmentSteps = 8;                               // 512 tokens between two promotions
 constexpr int kPlanes = 3;
 constexpr uint32_t kXBlockBytes = 32 * kStepTokens * 2;        // [32 features][64 tokens] bf16
 constexpr uint32_t kXPlaneBytes = kItemPairs * kXBlockBytes;

@@ -18,8 +18,9 @@ from .block_sparse import BlockSparseMatrix
 
 # Up to this many tokens inference computes from the stored blocks directly (``bsmm_gated_small``).  us, few-token kernel / weight
 # images and tensor-core kernel, on one B200: bf16, 4096 -> 8192 at density 0.25, 16 tokens 21 / 44, 32 tokens 26 / 44, 48 tokens
-# 42 / 44, 64 tokens 44 / 44; 4096 -> 16384 at 0.1, 32 tokens 29 / 32, 48 tokens 46 / 32; 1024 -> 2048 at 0.5, 32 tokens 12 / 15.
-# fp32, 4096 -> 8192: 16 tokens 40 / 98, 32 tokens 69 / 98, 48 tokens 99 / 98.
+# 42 / 44, 64 tokens 44 / 44; 4096 -> 16384 at 0.1, 32 tokens 29 / 32, 48 tokens 46 / 32; 1024 -> 2048 at 0.5, 32 tokens 8 / 15.
+# fp32, 4096 -> 8192: 8 tokens 23 / 88, 16 tokens 39 / 86, 32 tokens 68 / 75, 48 tokens 99 / 75; 1024 -> 4096 at 0.5, 16 tokens 14 / 31,
+# 32 tokens 24 / 23.
 SMALL_TOKENS = 32
 
 
