@@ -329,34 +329,35 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
  *   ptr / idx, plan            CSR of the 2 * hidden-row matrix, and bsmm_build_plan of it (FP32_SIMT: NULL)
  *   csc_ptr / csc_idx, csc_plan  the same of the CSC
  *   blocks, sddmm_plan         for the weight gradient, as bsmm_sddmm
- *   packed                     bsmm_packed_bytes bytes: written by the forward pass, read by the backward pass.  NULL where there is
- *                              none and the forward pass does not need them (see wgrad_plan)
- *   pre                        fp32 [m, 2 * hidden] for the backward pass; NULL where there is none and wgrad_plan is in use
+ *   packed                     bsmm_packed_bytes bytes: written by the forward pass, read by the backward pass
+ *   pre                        fp32 [m, 2 * hidden]: g and u, for the backward pass
+ *   dpre                       [m, 2 * hidden]: the backward pass's gradients of g and u
  *   flags                      precision, BSMM_DSD_GROUP(g) of `plan` (forward) or `csc_plan` (backward),
  *                              BSMM_GATED_PASS(activation and type flags as for bsmm_gated_act)
  *   dx, dw, dbias              NULL where not wanted; block_sumsq as bsmm_sddmm
- *   wgrad_plan                 bsmm_build_gated_wgrad_plan of the CSR, bsmm_gated_wgrad_plan_bytes bytes, 16-byte aligned, or NULL: with
- *                              it the forward pass and (from 64 tokens on) the weight gradient of fp32 tensors in BSMM_PREC_TF32X3
- *                              and BSMM_PREC_BF16X3 come from kernels that multiply three bf16 parts of every value and share the
- *                              input between gate and up blocks (relative error near 1e-6; magnitudes above bf16's largest
- *                              finite value, 3.39e38, round to infinity), the forward pass with the activation in the same
- *                              kernel; else from bsmm_dsd and bsmm_sddmm
+ *   f32_plan                   bsmm_build_gated_f32_plan of the CSR and CSC, bsmm_gated_f32_plan_bytes bytes, 16-byte aligned, or NULL.
+ *                              With it fp32 tensors in BSMM_PREC_TF32X3 and BSMM_PREC_BF16X3 go through kernels that multiply three
+ *                              bf16 parts of every value and share what gate and up blocks share (relative error near 1e-6;
+ *                              magnitudes above bf16's largest finite value, 3.39e38, count as infinite, and what an infinity reaches is
+ *                              NaN), the forward pass with the activation in the same kernel.  They use neither packed, plan and csc_plan, sddmm_plan and blocks nor
+ *                              dpre, which may be NULL, and pre may be NULL where no backward pass follows.  Without it the passes
+ *                              are made of bsmm_dsd, bsmm_sddmm and the activation's kernels
  *   workspace                  bsmm_gated_forward_workspace_bytes, bsmm_gated_backward_workspace_bytes bytes, 256-byte aligned
  */
 #define BSMM_GATED_PASS(f) (((uint32_t)(f)&0xFu) << 16)
 int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, int64_t nnz,
-                            const float* data, void* packed, const void* plan, const void* wgrad_plan, int64_t hidden,
+                            const float* data, void* packed, const void* plan, const void* f32_plan, int64_t hidden,
                             const float* bias, float* pre, void* h, void* workspace, uint32_t flags, bsmm_stream_t stream);
 int64_t bsmm_gated_forward_workspace_bytes(int64_t m, int64_t k, int64_t hidden, int64_t nnz, uint32_t flags);
 int64_t bsmm_gated_backward_workspace_bytes(int64_t m, int64_t k, int64_t hidden, int64_t nnz, uint32_t flags);
 int bsmm_gated_pass_backward(const void* x, const void* pre, const void* dh, int64_t m, int64_t k, const int32_t* idx,
                              const int32_t* csc_ptr, const int32_t* csc_idx, const int32_t* blocks, int64_t nnz,
                              const float* data, const void* packed, const void* csc_plan, const void* sddmm_plan,
-                             const void* wgrad_plan, int64_t hidden, void* dpre, void* dx, float* dw, float* dbias,
+                             const void* f32_plan, int64_t hidden, void* dpre, void* dx, float* dw, float* dbias,
                              float* block_sumsq, void* workspace, uint32_t flags, bsmm_stream_t stream);
-int64_t bsmm_gated_wgrad_plan_bytes(int64_t hidden, int64_t k, int64_t nnz);
-int bsmm_build_gated_wgrad_plan(const int32_t* ptr, const int32_t* idx, int64_t hidden, int64_t k, int64_t nnz, void* plan,
-                                bsmm_stream_t stream);
+int64_t bsmm_gated_f32_plan_bytes(int64_t hidden, int64_t k, int64_t nnz);
+int bsmm_build_gated_f32_plan(const int32_t* ptr, const int32_t* idx, const int32_t* csc_ptr, const int32_t* csc_idx, int64_t hidden,
+                              int64_t k, int64_t nnz, void* plan, bsmm_stream_t stream);
 
 /*
  * The gated block on bf16 tensors with bf16 products (fp32 sums) in one tensor-core kernel: both projections, the activation

@@ -16,7 +16,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(os.path.dirname(PKG_DIR), "include")
 LIB_PATH = os.path.join(PKG_DIR, "libbsmm_b200.so")
 SOURCES = ["bsmm_api.cu", "bsmm_simt.cu", "bsmm_pack.cu", "bsmm_plan.cu", "bsmm_pattern.cu", "bsmm_collective.cu", "bsmm_umma.cu", "bsmm_sddmm_umma.cu",
-           "bsmm_dropout.cu", "bsmm_gated.cu", "bsmm_gated_umma.cu", "bsmm_gated_f32.cu", "bsmm_gated_wgrad.cu", "bsmm_adapters.cu", "bsmm_adapters_umma.cu", "bsmm_feedforward_api.cu"]
+           "bsmm_dropout.cu", "bsmm_gated.cu", "bsmm_gated_umma.cu", "bsmm_gated_f32.cu", "bsmm_gated_wgrad.cu", "bsmm_gated_dgrad.cu", "bsmm_adapters.cu", "bsmm_adapters_umma.cu", "bsmm_feedforward_api.cu"]
 HEADERS = ["bsmm_common.cuh", "bsmm_umma.cuh", "bsmm_ptx.cuh", "bsmm_feedforward.cuh", "bsmm_adapters.cuh"]
 
 

@@ -129,7 +129,7 @@ cudaError_t launch_gated_act(const void* pre, int64_t m, int64_t hidden, void* h
 int64_t gated_act_workspace_bytes(int64_t m, int64_t hidden);
 cudaError_t launch_gated_act_backward(const void* pre, const void* dh, int64_t m, int64_t hidden, void* dpre,
                                       float* dbias, float* workspace, int act, bool pre_bf16, bool io_bf16,
-                                      void* planes, cudaStream_t stream);  // planes of dpre, or null (fp32 only)
+                                      void* planes, cudaStream_t stream);  // planes of dpre in its place, or null (fp32 only)
 cudaError_t launch_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx,
                                const float* data, int64_t nnz, int64_t hidden, const float* bias, void* h, int act,
                                bool x_bf16, bool h_bf16, cudaStream_t stream);
@@ -150,7 +150,7 @@ cudaError_t launch_gated_f32(const float* x, int64_t m, int64_t k, const float* 
                              const void* pairs_plan, int64_t hidden, const float* bias, float* h, float* pre, int act, void* workspace,
                              cudaStream_t stream);
 
-// The rows' pairs in the plan of bsmm_build_gated_wgrad_plan: a row's begin where its entries do in the CSR.
+// The rows' pairs in the plan of the weight gradient: a row's begin where its entries do in the CSR.
 struct GatedPairs {
     const int4* pairs;       // (input block, gate slot, up slot, 0), a slot -1 where that projection has no block
     const int32_t* counts;   // per pair-row
@@ -165,6 +165,14 @@ cudaError_t launch_split_planes(const float* x, int64_t m, int64_t k, void* plan
 int64_t gated_wgrad_workspace_bytes(int64_t hidden, int64_t nnz, int64_t tokens);
 cudaError_t launch_gated_wgrad(const void* x_planes, const void* d_planes, int64_t tokens, int64_t k, int64_t hidden, int64_t nnz,
                                const void* plan, float* out, float* block_sumsq, void* workspace, cudaStream_t stream);
+
+// the input gradient of fp32 tensors from the same planes (bsmm_gated_dgrad.cu)
+int64_t gated_dgrad_plan_bytes(int64_t k, int64_t nnz);
+cudaError_t launch_build_gated_dgrad_plan(const int32_t* col_ptr, const int32_t* col_idx, int64_t hidden, int64_t k, int64_t nnz, void* plan,
+                                          cudaStream_t stream);
+int64_t gated_dgrad_workspace_bytes(int64_t nnz);
+cudaError_t launch_gated_dgrad(const void* d_planes, int64_t m, int64_t k, int64_t hidden, int64_t nnz, const float* data,
+                               const int32_t* col_ptr, const void* plan, float* dx, void* workspace, cudaStream_t stream);
 
 struct AdapterCall {
     const void* x;           // [tokens, inner]

@@ -78,7 +78,6 @@ int bsmm_gated_small(const void* x, int64_t m, int64_t k, const int32_t* ptr, co
 static bool from_planes(int64_t nnz, uint32_t precision) {
     return nnz > 0 && (precision == BSMM_PREC_TF32X3 || precision == BSMM_PREC_BF16X3);
 }
-static bool wgrad_from_planes(int64_t m, int64_t nnz, uint32_t precision) { return m >= 64 && from_planes(nnz, precision); }
 static int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 int64_t bsmm_gated_forward_workspace_bytes(int64_t m, int64_t k, int64_t hidden, int64_t nnz, uint32_t flags) {
@@ -87,7 +86,7 @@ int64_t bsmm_gated_forward_workspace_bytes(int64_t m, int64_t k, int64_t hidden,
 }
 
 int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t* ptr, const int32_t* idx, int64_t nnz,
-                            const float* data, void* packed, const void* plan, const void* wgrad_plan, int64_t hidden,
+                            const float* data, void* packed, const void* plan, const void* f32_plan, int64_t hidden,
                             const float* bias, float* pre, void* h, void* workspace, uint32_t flags, bsmm_stream_t stream) {
     (void)cudaGetLastError();
     const uint32_t precision = flags & BSMM_PREC_MASK, pass = (flags >> 16) & 0xFu;
@@ -97,15 +96,15 @@ int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t*
         const int status = bsmm_pack_weights(data, nnz, precision, packed, nullptr, stream);
         if (status != BSMM_OK) return status;
     }
-    if (wgrad_plan != nullptr && pass == (pass & BSMM_GATED_GELU) && from_planes(nnz, precision)) {
+    if (f32_plan != nullptr && pass == (pass & BSMM_GATED_GELU) && from_planes(nnz, precision)) {
         if (m < 0 || k <= 0 || hidden < 0 || (hidden % 32) != 0 || (k % 32) != 0) return BSMM_ERR_INVALID_ARGUMENT;
         if (m == 0 || hidden == 0) return BSMM_OK;
         if (x == nullptr || ptr == nullptr || data == nullptr || h == nullptr || workspace == nullptr) return BSMM_ERR_INVALID_ARGUMENT;
-        if (!aligned(x, 16) || !aligned(ptr, 4) || !aligned(data, 16) || !aligned(wgrad_plan, 16) || !aligned(bias, 16) ||
+        if (!aligned(x, 16) || !aligned(ptr, 4) || !aligned(data, 16) || !aligned(f32_plan, 16) || !aligned(bias, 16) ||
             !aligned(pre, 16) || !aligned(h, 16) || !aligned(workspace, 256))
             return BSMM_ERR_INVALID_ARGUMENT;
         if (nnz > 0x7fffffff || k > BSMM_GATED_MAX_K || too_large(m, k) || too_large(m, 2 * hidden)) return BSMM_ERR_TOO_LARGE;
-        return bsmm::report_cuda(bsmm::launch_gated_f32(x, m, k, data, nnz, ptr, wgrad_plan, hidden, bias, static_cast<float*>(h), pre,
+        return bsmm::report_cuda(bsmm::launch_gated_f32(x, m, k, data, nnz, ptr, f32_plan, hidden, bias, static_cast<float*>(h), pre,
                                                         (pass & BSMM_GATED_GELU) != 0, workspace, static_cast<cudaStream_t>(stream)));
     }
     if (pre == nullptr && m > 0 && hidden > 0) return BSMM_ERR_INVALID_ARGUMENT;
@@ -119,33 +118,39 @@ int64_t bsmm_gated_backward_workspace_bytes(int64_t m, int64_t k, int64_t hidden
     const uint32_t precision = flags & BSMM_PREC_MASK;
     const int64_t a = bsmm_gated_act_workspace_bytes(m, hidden);
     if (k < 0 || too_large(m, k) || nnz < 0 || nnz > 0x7fffffff) return -1;
-    if (a >= 0 && wgrad_from_planes(m, nnz, precision)) {
-        const int64_t b = bsmm::gated_wgrad_workspace_bytes(hidden, nnz, m);
-        return padded(6 * bsmm::plane_pitch(m) * k) + padded(12 * bsmm::plane_pitch(m) * hidden) + (a > b ? a : b);
+    if (a >= 0 && m > 0 && from_planes(nnz, precision)) {
+        const int64_t b = bsmm::gated_wgrad_workspace_bytes(hidden, nnz, m), c = bsmm::gated_dgrad_workspace_bytes(nnz);
+        return padded(6 * bsmm::plane_pitch(m) * k) + padded(12 * bsmm::plane_pitch(m) * hidden) + (a > b ? (a > c ? a : c) : b > c ? b : c);
     }
     const int64_t b = bsmm_sddmm_workspace_bytes(2 * hidden, k, m, nnz, precision);
     return a < 0 || b < 0 ? -1 : a > b ? a : b;
 }
 
-int64_t bsmm_gated_wgrad_plan_bytes(int64_t hidden, int64_t k, int64_t nnz) {
+int64_t bsmm_gated_f32_plan_bytes(int64_t hidden, int64_t k, int64_t nnz) {
     if (bsmm_gated_plan_bytes(hidden, k, nnz) < 0) return -1;
-    return bsmm::gated_wgrad_plan_bytes(hidden, nnz);
+    return padded(bsmm::gated_wgrad_plan_bytes(hidden, nnz)) + bsmm::gated_dgrad_plan_bytes(k, nnz);
 }
 
-int bsmm_build_gated_wgrad_plan(const int32_t* ptr, const int32_t* idx, int64_t hidden, int64_t k, int64_t nnz, void* plan,
-                                bsmm_stream_t stream) {
+int bsmm_build_gated_f32_plan(const int32_t* ptr, const int32_t* idx, const int32_t* csc_ptr, const int32_t* csc_idx, int64_t hidden,
+                              int64_t k, int64_t nnz, void* plan, bsmm_stream_t stream) {
     (void)cudaGetLastError();
-    if (bsmm_gated_plan_bytes(hidden, k, nnz) < 0 || ptr == nullptr || plan == nullptr || (nnz > 0 && idx == nullptr) ||
-        !aligned(ptr, 4) || !aligned(idx, 8) || !aligned(plan, 16))
+    if (bsmm_gated_plan_bytes(hidden, k, nnz) < 0 || ptr == nullptr || csc_ptr == nullptr || plan == nullptr ||
+        (nnz > 0 && (idx == nullptr || csc_idx == nullptr)) || !aligned(ptr, 4) || !aligned(idx, 8) || !aligned(csc_ptr, 4) ||
+        !aligned(csc_idx, 8) || !aligned(plan, 16))
         return BSMM_ERR_INVALID_ARGUMENT;
     if (k > BSMM_GATED_MAX_K) return BSMM_ERR_TOO_LARGE;
-    return bsmm::report_cuda(bsmm::launch_build_gated_wgrad_plan(ptr, idx, hidden, k, nnz, plan, static_cast<cudaStream_t>(stream)));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t err = bsmm::launch_build_gated_wgrad_plan(ptr, idx, hidden, k, nnz, plan, s);
+    if (err == cudaSuccess)
+        err = bsmm::launch_build_gated_dgrad_plan(csc_ptr, csc_idx, hidden, k, nnz,
+                                                  static_cast<uint8_t*>(plan) + padded(bsmm::gated_wgrad_plan_bytes(hidden, nnz)), s);
+    return bsmm::report_cuda(err);
 }
 
 int bsmm_gated_pass_backward(const void* x, const void* pre, const void* dh, int64_t m, int64_t k, const int32_t* idx,
                              const int32_t* csc_ptr, const int32_t* csc_idx, const int32_t* blocks, int64_t nnz,
                              const float* data, const void* packed, const void* csc_plan, const void* sddmm_plan,
-                             const void* wgrad_plan, int64_t hidden, void* dpre, void* dx, float* dw, float* dbias,
+                             const void* f32_plan, int64_t hidden, void* dpre, void* dx, float* dw, float* dbias,
                              float* block_sumsq, void* workspace, uint32_t flags, bsmm_stream_t stream) {
     (void)cudaGetLastError();
     const uint32_t precision = flags & BSMM_PREC_MASK, pass = (flags >> 16) & 0xFu;
@@ -155,29 +160,32 @@ int bsmm_gated_pass_backward(const void* x, const void* pre, const void* dh, int
     if (io16 && (precision != BSMM_PREC_BF16 || m < 32 || nnz == 0)) return BSMM_ERR_UNSUPPORTED;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     // the weight gradient before the input gradient: in data-parallel training its all-reduce can overlap the latter
-    int status = BSMM_OK;
-    if (dw != nullptr && wgrad_plan != nullptr && !io16 && wgrad_from_planes(m, nnz, precision)) {
-        if (m < 0 || hidden <= 0 || k <= 0 || (hidden % 32) != 0 || (k % 32) != 0 || x == nullptr || pre == nullptr || dh == nullptr ||
-            dpre == nullptr || workspace == nullptr || !aligned(x, 16) || !aligned(pre, 16) || !aligned(dh, 16) || !aligned(dpre, 16) ||
-            !aligned(dw, 16) || !aligned(dbias, 4) || !aligned(wgrad_plan, 16) || !aligned(workspace, 256))
+    if (f32_plan != nullptr && !io16 && m > 0 && from_planes(nnz, precision)) {
+        if (hidden <= 0 || k <= 0 || (hidden % 32) != 0 || (k % 32) != 0 || x == nullptr || pre == nullptr || dh == nullptr || workspace == nullptr ||
+            (dx != nullptr && (csc_ptr == nullptr || data == nullptr)) || !aligned(x, 16) || !aligned(pre, 16) || !aligned(dh, 16) ||
+            !aligned(csc_ptr, 4) || !aligned(data, 16) || !aligned(dx, 16) || !aligned(dw, 16) || !aligned(dbias, 4) || !aligned(f32_plan, 16) ||
+            !aligned(workspace, 256))
             return BSMM_ERR_INVALID_ARGUMENT;
         if (gated_types(pass) != BSMM_OK || (pass & BSMM_GATED_X_BF16) != 0) return BSMM_ERR_UNSUPPORTED;
         if (nnz > 0x7fffffff || k > BSMM_GATED_MAX_K || too_large(m, k) || too_large(m, 2 * hidden)) return BSMM_ERR_TOO_LARGE;
         uint8_t* x_planes = static_cast<uint8_t*>(workspace);
         uint8_t* d_planes = x_planes + padded(6 * bsmm::plane_pitch(m) * k);
-        uint8_t* rest = d_planes + padded(12 * bsmm::plane_pitch(m) * hidden);
-        cudaError_t err = bsmm::launch_gated_act_backward(pre, dh, m, hidden, dpre, dbias, reinterpret_cast<float*>(rest),
+        uint8_t* rest = d_planes + padded(12 * bsmm::plane_pitch(m) * hidden);  // of each step in turn
+        cudaError_t err = bsmm::launch_gated_act_backward(pre, dh, m, hidden, nullptr, dbias, reinterpret_cast<float*>(rest),
                                                           (pass & BSMM_GATED_GELU) != 0, false, false, d_planes, s);
-        if (err == cudaSuccess) err = bsmm::launch_split_planes(static_cast<const float*>(x), m, k, x_planes, s);
-        if (err == cudaSuccess)
-            err = bsmm::launch_gated_wgrad(x_planes, d_planes, m, k, hidden, nnz, wgrad_plan, dw, block_sumsq, rest, s);
-        status = bsmm::report_cuda(err);
-    } else {
-        status = bsmm_gated_act_backward(pre, dh, m, hidden, dpre, dbias, workspace, pass, stream);
-        if (status == BSMM_OK && dw != nullptr)
-            status = bsmm_sddmm(dpre, x, 2 * hidden, k, m, dw, blocks, nnz, idx, sddmm_plan, block_sumsq, workspace,
-                                precision | (io16 ? BSMM_SDDMM_IO_BF16 : 0u), stream);
+        if (err == cudaSuccess && dw != nullptr) err = bsmm::launch_split_planes(static_cast<const float*>(x), m, k, x_planes, s);
+        if (err == cudaSuccess && dw != nullptr)
+            err = bsmm::launch_gated_wgrad(x_planes, d_planes, m, k, hidden, nnz, f32_plan, dw, block_sumsq, rest, s);
+        if (err == cudaSuccess && dx != nullptr)
+            err = bsmm::launch_gated_dgrad(d_planes, m, k, hidden, nnz, data, csc_ptr,
+                                           static_cast<const uint8_t*>(f32_plan) + padded(bsmm::gated_wgrad_plan_bytes(hidden, nnz)),
+                                           static_cast<float*>(dx), rest, s);
+        return bsmm::report_cuda(err);
     }
+    int status = bsmm_gated_act_backward(pre, dh, m, hidden, dpre, dbias, workspace, pass, stream);
+    if (status == BSMM_OK && dw != nullptr)
+        status = bsmm_sddmm(dpre, x, 2 * hidden, k, m, dw, blocks, nnz, idx, sddmm_plan, block_sumsq, workspace,
+                            precision | (io16 ? BSMM_SDDMM_IO_BF16 : 0u), stream);
     if (status == BSMM_OK && dx != nullptr)
         status = bsmm_dsd(dpre, m, 2 * hidden, csc_ptr, csc_idx, nnz, data, packed, csc_plan, k, dx, nullptr,
                           (flags & (BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF))) | BSMM_DSD_DGRAD | (io16 ? BSMM_DSD_IO_BF16 : 0u), stream);

@@ -14,13 +14,13 @@
 //   warp 0 loads, warp 1 issues, warps 2-9 read out (four per half), the sums and h through shared memory in whole lines.
 // Bound by the tensor cores.  8192 tokens, 4096 -> 2 x 4096 at density 0.25 with g and u kept: 720 us, 1145 TFLOP/s (713 with
 // segments of 32 pairs, but a relative error of 1.8e-6 instead of 0.9e-6; 759 with each lane storing its own token) + 52 to split
-// x + 19 for the images; bsmm_dsd in TF32x3 and bsmm_gated_act as kernels of their own take 941.
+// x + 19 for the images; bsmm_dsd in TF32x3 and
+// bsmm_gated_act as kernels of their own take 941.
 // Without g and u kept, TF32x3 products before -> this kernel, us (device, images and split included):
 //   4096 tokens, 1024 -> 2 x 4096 at 0.5: 230 -> 185   512: 70 -> 41   64: 39 -> 23
 //   4096 tokens, 8192 -> 2 x 2048 at 0.25: 414 -> 400  512: 93 -> 81   64: 91 -> 53
 //   4096 tokens, 512 -> 2 x 512 at 0.5: 40 -> 28       512: 19 -> 16   64: 20 -> 16
-// With them kept the backward pass's images are made here too, and few tokens cost up to a quarter more (8192 -> 2 x 2048, 512 tokens:
-// 93 -> 115) or less (2048 -> 2 x 8192: 66 -> 61); the relative error falls from about 4e-6 to 8e-7 throughout.
+// The relative error falls from about 4e-6 to 8e-7 throughout.
 // Every wait is bounded; on expiry the CTA raises the device status word and drains.
 #include <cuda_bf16.h>
 

@@ -11,7 +11,7 @@
 // sums are added in fp32 registers (segments of 1024: 757 us instead of 772 on the case below, error 1.6e-6 instead of 1.05e-6).
 //
 // The three parts are written beforehand as three bf16 matrices ("planes"), transposed: [features][tokens], for x by
-// split_planes_kernel and for [dg | du] by the activation's backward kernel: tokens are the contraction index, and rows of
+// split_planes_kernel and for [dg | du], which the input gradient reads too, by the activation's backward kernel: tokens are the contraction index, and rows of
 // 64 tokens are what TMA and the tensor core move as one 128-byte line.
 //
 // CTA = one item (up to 4 pairs of one pair-row, which fill the 128 rows of an instruction) x one range of tokens.  Per 64 tokens:

@@ -58,8 +58,8 @@ EXPORTS = (
     "bsmm_gated_forward_workspace_bytes",
     "bsmm_gated_backward_workspace_bytes",
     "bsmm_gated_pass_backward",
-    "bsmm_gated_wgrad_plan_bytes",
-    "bsmm_build_gated_wgrad_plan",
+    "bsmm_gated_f32_plan_bytes",
+    "bsmm_build_gated_f32_plan",
     "bsmm_gated_plan_bytes",
     "bsmm_gated_images_bytes",
     "bsmm_build_gated_plan",
@@ -159,10 +159,10 @@ def load():
     lib.bsmm_gated_pass_backward.restype = i32
     lib.bsmm_gated_pass_backward.argtypes = [vp, vp, vp, i64, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp,
                                              vp, vp, u32, vp]
-    lib.bsmm_gated_wgrad_plan_bytes.restype = i64
-    lib.bsmm_gated_wgrad_plan_bytes.argtypes = [i64, i64, i64]
-    lib.bsmm_build_gated_wgrad_plan.restype = i32
-    lib.bsmm_build_gated_wgrad_plan.argtypes = [vp, vp, i64, i64, i64, vp, vp]
+    lib.bsmm_gated_f32_plan_bytes.restype = i64
+    lib.bsmm_gated_f32_plan_bytes.argtypes = [i64, i64, i64]
+    lib.bsmm_build_gated_f32_plan.restype = i32
+    lib.bsmm_build_gated_f32_plan.argtypes = [vp, vp, vp, vp, i64, i64, i64, vp, vp]
     lib.bsmm_gated_plan_bytes.restype = i64
     lib.bsmm_gated_plan_bytes.argtypes = [i64, i64, i64]
     lib.bsmm_gated_images_bytes.restype = i64
@@ -672,12 +672,12 @@ class GatedPass:
         self.sddmm = SddmmPlan(ptr, idx)
         self.blocks = _aligned(blocks, 8)
         lib, hidden, k = load(), self.csr.n_out_blocks * 16, self.csc.n_out_blocks * 32
-        self.wgrad = None
+        self.f32 = None
         if k <= GATED_MAX_K:
-            self.wgrad = torch.empty(lib.bsmm_gated_wgrad_plan_bytes(hidden, k, self.csr.nnz), dtype=torch.uint8, device=ptr.device)
+            self.f32 = torch.empty(lib.bsmm_gated_f32_plan_bytes(hidden, k, self.csr.nnz), dtype=torch.uint8, device=ptr.device)
             with _on(ptr.device):
-                check(lib.bsmm_build_gated_wgrad_plan(_ptr(self.csr.ptr), _ptr(self.csr.idx), hidden, k, self.csr.nnz,
-                                                      _ptr(self.wgrad), _stream(ptr.device)), "bsmm_build_gated_wgrad_plan")
+                check(lib.bsmm_build_gated_f32_plan(_ptr(self.csr.ptr), _ptr(self.csr.idx), _ptr(self.csc.ptr), _ptr(self.csc.idx), hidden, k,
+                                                    self.csr.nnz, _ptr(self.f32), _stream(ptr.device)), "bsmm_build_gated_f32_plan")
         self.built, self.groups = _Built(), set()
         with _on(ptr.device):
             self.built.mark(ptr.device)
@@ -693,14 +693,14 @@ class GatedPass:
         return group, buffer
 
     def forward(self, x, data, bias, activation, precision, out_dtype, keep=True):
-        """``(h, pre, packed)`` of a contiguous fp32 ``x``: for backward (``keep``) ``pre`` in fp32 and the weight images (``None`` for
-        exact fp32)."""
+        """``(h, pre, packed)`` of a contiguous fp32 ``x``: for backward (``keep``) ``pre`` in fp32 and the weight images (``None`` where
+        there is no use for them)."""
         _need_cuda(x, "x")
         lib, csr, device = load(), self.csr, x.device
         m, k = x.shape
         hidden = csr.n_out_blocks * 16
         flags = precision | (_gated_flags(activation) | (GATED_IO_BF16 if out_dtype is torch.bfloat16 else 0)) << 16
-        ws_bytes = lib.bsmm_gated_forward_workspace_bytes(m, k, hidden, csr.nnz, flags) if self.wgrad is not None else 0
+        ws_bytes = lib.bsmm_gated_forward_workspace_bytes(m, k, hidden, csr.nnz, flags) if self.f32 is not None else 0
         whole = ws_bytes > 0  # one kernel for projections, activation and product
         h = torch.empty((m, hidden), dtype=out_dtype, device=device)
         pre = torch.empty((m, 2 * hidden), dtype=torch.float32, device=device) if keep or not whole else None
@@ -710,15 +710,15 @@ class GatedPass:
         elif precision != PREC_FP32_SIMT:
             group, plan = self._buffer(csr, m, precision, device)
             flags |= group << 8
-        if precision != PREC_FP32_SIMT and (keep or not whole):
+        if precision != PREC_FP32_SIMT and not whole:
             packed = torch.empty(max(16, lib.bsmm_packed_bytes(csr.nnz, precision)), dtype=torch.uint8, device=device)
         x, data, bias = _aligned(x), _aligned(data), _aligned(bias)
         with _on(device):
-            self.built.join(_stream(device), device, (plan, self.wgrad))
+            self.built.join(_stream(device), device, (plan, self.f32))
             check(
                 lib.bsmm_gated_pass_forward(
                     x.data_ptr(), m, k, csr.ptr.data_ptr(), csr.idx.data_ptr(), csr.nnz, data.data_ptr(), _ptr(packed), _ptr(plan),
-                    _ptr(self.wgrad) if whole else None, hidden, _ptr(bias), _ptr(pre), h.data_ptr(), _ptr(ws), flags, _stream(device)),
+                    _ptr(self.f32) if whole else None, hidden, _ptr(bias), _ptr(pre), h.data_ptr(), _ptr(ws), flags, _stream(device)),
                 "bsmm_gated_pass_forward",
             )
         return h, pre, packed
@@ -728,7 +728,8 @@ class GatedPass:
         lib, csc, device = load(), self.csc, dh.device
         m, hidden = dh.shape
         k = csc.n_out_blocks * 32
-        dpre = torch.empty((m, 2 * hidden), dtype=dh.dtype, device=device)
+        planes = self.f32 is not None and precision in (PREC_TF32X3, PREC_BF16X3) and m > 0 and csc.nnz > 0
+        dpre = None if planes else torch.empty((m, 2 * hidden), dtype=dh.dtype, device=device)
         dx = torch.empty((m, k), dtype=dh.dtype, device=device) if want_x else None
         dw = torch.empty_like(data) if want_w else None
         sumsq = torch.empty(csc.nnz, dtype=torch.float32, device=device) if want_w else None
@@ -737,17 +738,17 @@ class GatedPass:
         flags = precision | (_gated_flags(activation) | types) << 16
         ws = torch.empty(max(16, lib.bsmm_gated_backward_workspace_bytes(m, k, hidden, csc.nnz, flags)), dtype=torch.uint8, device=device)
         plan = None
-        if precision != PREC_FP32_SIMT and want_x:
+        if precision != PREC_FP32_SIMT and want_x and not planes:
             group, plan = self._buffer(csc, m, precision, device)
             flags |= group << 8
         x, dh, data = _aligned(x), _aligned(dh), _aligned(data)
         with _on(device):
-            self.built.join(_stream(device), device, (plan, self.wgrad, self.sddmm.buffer))
+            self.built.join(_stream(device), device, (plan, self.f32, self.sddmm.buffer))
             check(
                 lib.bsmm_gated_pass_backward(
                     x.data_ptr(), pre.data_ptr(), dh.data_ptr(), m, k, self.sddmm.idx.data_ptr(), csc.ptr.data_ptr(),
                     csc.idx.data_ptr(), self.blocks.data_ptr(), csc.nnz, data.data_ptr(), _ptr(packed), _ptr(plan),
-                    self.sddmm.buffer.data_ptr(), _ptr(self.wgrad), hidden, dpre.data_ptr(), _ptr(dx), _ptr(dw), _ptr(dbias), _ptr(sumsq),
+                    self.sddmm.buffer.data_ptr(), _ptr(self.f32) if planes else None, hidden, _ptr(dpre), _ptr(dx), _ptr(dw), _ptr(dbias), _ptr(sumsq),
                     ws.data_ptr(), flags, _stream(device)),
                 "bsmm_gated_pass_backward",
             )

@@ -57,7 +57,7 @@ def test_gated_kernel_entry_points():
     assert run(fake, 4, 32, fake, odd, 1, 32, null, fake, null, both, null) == INVALID
     assert run(fake, 4, native.GATED_MAX_K + 32, fake, fake, 1, 32, null, fake, null, both, null) == TOO_LARGE
     assert run(null, 0, 32, null, null, 0, 32, null, null, null, both, null) == OK
-    assert lib.bsmm_build_gated_wgrad_plan(fake, fake, 32, 48, 1, fake, null) == INVALID
+    assert lib.bsmm_build_gated_f32_plan(fake, fake, fake, fake, 32, 48, 1, fake, null) == INVALID
     passes = lib.bsmm_gated_pass_forward
     x3 = native.PREC_TF32X3
     assert passes(fake, 4, 32, fake, fake, 1, fake, null, null, null, 32, null, fake, fake, null, 1 << 30, null) == UNSUPPORTED

@@ -418,13 +418,41 @@ def test_the_fp32_kernel_alone(act, tokens, inner, hidden, density, same):
     passes = gated_linear._gated_pass(layer.weight)
     data, bias = layer.weight.data.detach(), layer.bias.detach()
     h, pre, packed = passes.forward(x.cuda(), data, bias, act, native.PREC_TF32X3, torch.float32)
-    assert packed is not None and torch.isfinite(pre).all()
+    assert packed is None and torch.isfinite(pre).all()
     want = x.double() @ layer.weight.to_dense().detach().cpu().double().t() + bias.cpu().double()
     assert rel(pre, want) <= 2e-6
     assert rel(h, reference(layer, x)) <= 6e-6
     alone = passes.forward(x.cuda(), data, bias, act, native.PREC_TF32X3, torch.float32, keep=False)
-    assert alone[1] is None and alone[2] is None and torch.equal(alone[0], h)
+    assert alone[1] is None and torch.equal(alone[0], h)
     assert torch.equal(native.gated_act(pre, act, torch.float32), h)
+    assert_device_healthy()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("tokens,inner,hidden,density,same", [
+    (1, 32, 32, 1.0, True), (33, 96, 64, 1.0, True), (64, 160, 544, 0.5, False), (129, 96, 1056, 0.4, True), (257, 2080, 64, 0.3, False),
+    (1000, 96, 4096, 0.9, True), (700, 4096, 64, 0.6, False), (2500, 1056, 1184, 0.2, True), (300, 64, 32 * 1100, 0.05, False),
+    (128 * 149 + 1, 32, 64, 1.0, True), (5000, 4096, 96, 0.02, False),
+])
+def test_the_fp32_input_gradient(act, tokens, inner, hidden, density, same):
+    """Three bf16 parts of every value, as the weight gradient: 2e-6 of the norm.  Columns without a block get zeros."""
+    g = torch.Generator().manual_seed(tokens)
+    mask = torch.rand((hidden // 16, inner // 32), generator=g) < density
+    if same:
+        mask[1::2] = mask[0::2]
+    mask[0, 0] = True
+    layer = make(inner, hidden, act=act, mask=mask, seed=tokens)
+    passes = gated_linear._gated_pass(layer.weight)
+    x, pre, dh = randn((tokens, inner), 1).cuda(), randn((tokens, 2 * hidden), 2).cuda(), randn((tokens, hidden), 3).cuda()
+    data = layer.weight.data.detach()
+    got = passes.backward(x, pre, dh, data, None, act, native.PREC_TF32X3, True, False, False)
+    dpre, _ = native.gated_act_backward(pre, dh, act, False)
+    want = dpre.cpu().double() @ layer.weight.to_dense().detach().cpu().double()
+    assert got[1] is None and got[2] is None and torch.isfinite(got[0]).all()
+    assert rel(got[0], want) <= 2e-6
+    assert (got[0].cpu()[want == 0] == 0).all()
+    again = passes.backward(x, pre, dh, data, None, act, native.PREC_BF16X3, True, True, True)
+    assert torch.equal(again[0], got[0])
     assert_device_healthy()
 
 
