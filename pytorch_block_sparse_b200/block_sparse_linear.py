@@ -20,7 +20,7 @@ import torch.autograd
 import torch.nn as nn
 
 from . import native
-from .dropout import dropout_residual, new_rng_state, next_rng, rate_units
+from .dropout import dropout_residual, rate_units
 from .block_sparse import BlockSparseMatrix, BlockSparseMatrixBase, BlockSparseMatrixEmulator
 
 
@@ -101,8 +101,7 @@ class BlockSparseLinear(nn.Module):
     everything but 32x32 there).  Parameters live on ``"cuda"``.
 
     Not in the reference: ``activation`` (``"gelu"``, in the forward kernel's epilogue) and ``dropout``, the rate of a dropout of
-    the output in training mode, before the residual is added; its mask comes from a counter-based generator whose
-    state (a seed from torch's default generator, a counter) lives on the device and is not part of the state dict.
+    the output in training mode, before the residual is added (``dropout_residual``, its mask drawn from torch's generator).
     """
 
     OPTIMIZED_BLOCK_SIZE = 32
@@ -171,8 +170,6 @@ class BlockSparseLinear(nn.Module):
                     self.bias.copy_(torch_nn_linear.bias)
         else:
             self.register_parameter("bias", None)
-        if rate_units(dropout) > 0:
-            self.register_buffer("dropout_rng", new_rng_state("cuda"), persistent=False)
 
     def forward(self, x, residual=None, adapters=None):
         """``act(x @ W.T + bias + residual)``; ``residual`` (not in the reference) has the output's shape and is
@@ -193,7 +190,7 @@ class BlockSparseLinear(nn.Module):
         if residual is not None:
             wide = torch.promote_types(y.dtype, residual.dtype)
             y, residual = y.to(wide), residual.to(wide).expand_as(y)
-        return dropout_residual(y, self.dropout, next_rng(self.dropout_rng), residual=residual)
+        return dropout_residual(y, self.dropout, residual=residual)
 
     def _forward_adapters(self, x, residual, adapters, requests):
         if adapters.in_features != self.in_features or adapters.out_features != self.out_features:

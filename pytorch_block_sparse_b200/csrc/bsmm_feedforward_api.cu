@@ -92,10 +92,6 @@ int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t*
     const uint32_t precision = flags & BSMM_PREC_MASK, pass = (flags >> 16) & 0xFu;
     if ((flags & ~(BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF) | BSMM_GATED_PASS(0xF))) != 0 || (pass & BSMM_GATED_PRE_BF16) != 0)
         return BSMM_ERR_UNSUPPORTED;
-    if (precision != BSMM_PREC_FP32_SIMT && packed != nullptr) {
-        const int status = bsmm_pack_weights(data, nnz, precision, packed, nullptr, stream);
-        if (status != BSMM_OK) return status;
-    }
     if (f32_plan != nullptr && pass == (pass & BSMM_GATED_GELU) && from_planes(nnz, precision)) {
         if (m < 0 || k <= 0 || hidden < 0 || (hidden % 32) != 0 || (k % 32) != 0) return BSMM_ERR_INVALID_ARGUMENT;
         if (m == 0 || hidden == 0) return BSMM_OK;
@@ -108,6 +104,10 @@ int bsmm_gated_pass_forward(const float* x, int64_t m, int64_t k, const int32_t*
                                                         (pass & BSMM_GATED_GELU) != 0, workspace, static_cast<cudaStream_t>(stream)));
     }
     if (pre == nullptr && m > 0 && hidden > 0) return BSMM_ERR_INVALID_ARGUMENT;
+    if (precision != BSMM_PREC_FP32_SIMT) {
+        const int status = bsmm_pack_weights(data, nnz, precision, packed, nullptr, stream);
+        if (status != BSMM_OK) return status;
+    }
     const int status = bsmm_dsd(x, m, k, ptr, idx, nnz, data, packed, plan, 2 * hidden, pre, bias,
                                 flags & (BSMM_PREC_MASK | BSMM_DSD_GROUP(0xFF)), stream);
     return status != BSMM_OK ? status : bsmm_gated_act(pre, m, hidden, h, pass, stream);

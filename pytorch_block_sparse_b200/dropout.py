@@ -45,12 +45,14 @@ class DropoutResidualFunction(torch.autograd.Function):
         return dx, grad if want_residual else None, None, None
 
 
-def dropout_residual(x, p, rng, residual=None):
+def dropout_residual(x, p, rng=None, residual=None):
     """``dropout(x, p) + residual`` in one kernel, mask never stored.
 
     ``x``: fp32 or bf16 CUDA tensor; ``residual`` (optional): same shape and type.  ``rng``: int64 ``[2]`` CUDA tensor (seed,
     counter) -- equal values give equal masks; it is read when the kernel runs, so a captured call draws anew in every
     replay if the graph moves the counter on (:func:`next_rng`), and it must not change between forward and backward.
+    Without one both numbers are drawn from torch's generator of ``x``'s device: seeds, activation checkpointing and captured
+    graphs then behave as with torch's own dropout.
     Element ``i`` (of the contiguous tensor) is kept when its 16-bit number of Philox4x32-10 is at least ``round(p * 65536)``;
     kept values are scaled by the inverse of the exact share kept.  A dropped value leaves exactly the residual, also where
     ``x`` is infinite or NaN."""
@@ -62,7 +64,9 @@ def dropout_residual(x, p, rng, residual=None):
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError("residual must match x: %s %s %s, got %s %s %s" % (
             tuple(x.shape), x.dtype, x.device, tuple(residual.shape), residual.dtype, residual.device))
-    if rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or rng.device != x.device or not rng.is_contiguous():
+    if rng is None:
+        rng = torch.randint(1 << 62, (2,), device=x.device)
+    elif rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or rng.device != x.device or not rng.is_contiguous():
         raise ValueError("rng must be a contiguous int64 tensor of 2 elements (seed, counter) on %s" % x.device)
     return DropoutResidualFunction.apply(x, residual, cut, rng)
 

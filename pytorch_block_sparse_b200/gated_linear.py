@@ -45,8 +45,7 @@ class BlockSparseGatedFunction(torch.autograd.Function):
         assert weight_data.is_contiguous()
         ctx.weight, ctx.activation = weight, activation
         ctx.precision = prec = native.resolve_precision(precision)
-        # The weights are packed once per forward, never cached (writes through ``.data`` do not bump version counters);
-        # backward uses the images made here: the weights that the forward saw.
+        # The weights are packed in every pass, never cached (writes through ``.data`` do not bump version counters).
         if _fused(input, prec):
             # g and u are kept in bf16, the type of every other tensor that this mode keeps for backward
             h, pre = native.gated_forward(input, _gated_plan(weight), weight_data, bias, activation, True)
@@ -117,7 +116,9 @@ class BlockSparseGatedLinear(nn.Module):
     ``[2 * hidden, in]`` with alternating block-rows and any pattern.  ``activation``: ``"silu"`` or ``"gelu"`` (erf form).
     ``bias``: fp32 ``[2 * hidden]``, laid out like the weight's rows.  ``precision``: as ``set_default_precision``; ``None`` follows the
     default at each call.  Input: fp32 or bf16 ``[..., in]``; the output is bf16 for bf16 input in the ``"bf16"`` precision, else
-    fp32.  Without gradients and up to ``SMALL_TOKENS`` tokens the products are exact fp32 in every precision."""
+    fp32.  Without gradients and up to ``SMALL_TOKENS`` tokens the products are exact fp32 in every precision.  In the fp32-class
+    precisions (``"tf32x3"``, ``"bf16x3"``) a pass needs a workspace of 6 bytes per input value, backward 12 more per hidden unit
+    and token."""
 
     def __init__(self, in_features, hidden_features, bias=True, density=0.5, activation="silu", weight=None, precision=None):
         super().__init__()

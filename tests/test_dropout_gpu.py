@@ -1,8 +1,11 @@
 """Dropout from the counter-based generator with the residual add: the mask against a numpy statement of Philox4x32-10
 bit by bit, values against 64 bits, the gradient, streams, graphs and the layer that carries it."""
+import copy
+
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from pytorch_block_sparse_b200 import BlockSparseLinear, dropout_residual, new_rng_state, next_rng
 
@@ -180,13 +183,15 @@ def test_the_layer_drops_its_output_in_training_only():
         lin.weight.data.normal_(0, 0.1)
         lin.bias.normal_()
     x, residual, dy = randn((4, 9, 128), 1).cuda(), randn((4, 9, 96), 2).cuda(), randn((4, 9, 96), 3).cuda()
-    assert "dropout_rng" not in lin.state_dict()
+    assert sorted(lin.state_dict()) == sorted(BlockSparseLinear(128, 96, density=0.5).state_dict())
     plain = BlockSparseLinear(128, 96, density=0.5)
     plain.weight, plain.bias = lin.weight, lin.bias
-    seed = lin.dropout_rng.tolist()[0]
+    torch.manual_seed(3)
+    seed, counter = torch.randint(1 << 62, (2,), device="cuda").tolist()
+    torch.manual_seed(3)
     xa, ra = x.clone().requires_grad_(), residual.clone().requires_grad_()
     out = lin(xa, residual=ra)
-    keep = torch.from_numpy(philox_halves(out.numel(), seed, 0) >= 16384).view(out.shape).cuda()
+    keep = torch.from_numpy(philox_halves(out.numel(), seed, counter) >= 16384).view(out.shape).cuda()
     xb = x.clone().requires_grad_()
     y = plain(xb)
     want = torch.where(keep, y * (65536 / 49152), 0.0) + residual
@@ -196,7 +201,36 @@ def test_the_layer_drops_its_output_in_training_only():
     assert torch.equal(got[1], dy)
     for a, b in zip((got[0], got[2], got[3]), ref):
         assert torch.allclose(a, b, rtol=1e-5, atol=1e-5)
-    assert lin.dropout_rng.tolist() == [seed, 1]
     lin.eval()
     assert torch.equal(lin(x, residual=residual), plain(x, residual=residual))
-    assert lin.dropout_rng.tolist() == [seed, 1]
+
+
+def test_checkpointed_copied_and_captured_layers():
+    """What torch's own dropout does: a recomputed forward pass draws the same mask again, a copy of a layer draws others than
+    the layer, a captured step draws anew in every replay."""
+    np.random.seed(0)
+    torch.manual_seed(0)
+    lin = BlockSparseLinear(64, 64, density=1.0, dropout=0.5)
+    with torch.no_grad():
+        lin.weight.data.normal_(0, 0.1)
+    x = randn((100, 64), 1).cuda().requires_grad_()
+    torch.manual_seed(7)
+    (want,) = torch.autograd.grad(lin(x).square().sum(), x)
+    torch.manual_seed(7)
+    (got,) = torch.autograd.grad(torch.utils.checkpoint.checkpoint(lin, x, use_reentrant=False).square().sum(), x)
+    assert torch.equal(got, want)
+    torch.manual_seed(7)
+    assert not torch.equal(lin(x) == 0, copy.deepcopy(lin)(x) == 0)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(stream):
+        lin(x)
+    torch.cuda.synchronize()
+    with torch.no_grad(), torch.cuda.graph(graph, stream=stream):
+        out = lin(x)
+    masks = []
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        masks.append((out == 0).cpu())
+    assert not torch.equal(*masks) and 0.4 < masks[0].float().mean().item() < 0.6

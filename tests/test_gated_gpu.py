@@ -1,5 +1,7 @@
 """The gated feed-forward block: the activation kernels elementwise, the layer in every precision against 64 bits (values and
 gradients), few tokens, odd patterns, graphs and streams, and a feed-forward block built of it."""
+import copy
+import io
 import math
 
 import numpy as np
@@ -7,7 +9,7 @@ import pytest
 import torch
 
 from pytorch_block_sparse_b200 import (AdapterRequests, BlockSparseGatedLinear, BlockSparseLinear, BlockSparseMatrix,
-                                       LowRankAdapters, native)
+                                       LowRankAdapters, SparseOptimizer, native)
 from pytorch_block_sparse_b200 import gated_linear
 from pytorch_block_sparse_b200.gated_linear import SMALL_TOKENS, interleave_rows, split_rows
 
@@ -456,6 +458,47 @@ def test_the_fp32_input_gradient(act, tokens, inner, hidden, density, same):
     assert_device_healthy()
 
 
+@pytest.mark.parametrize("precision", ["tf32x3", "fp32", "bf16"])
+def test_no_tokens_with_gradients(precision):
+    layer = make(64, 96, precision=precision)
+    x = torch.empty((2, 0, 64), device="cuda", dtype=torch.bfloat16 if precision == "bf16" else torch.float32, requires_grad=True)
+    h = layer(x)
+    assert h.shape == (2, 0, 96)
+    got = torch.autograd.grad(h.sum(), [x, layer.weight.data, layer.bias])
+    assert got[0].shape == x.shape and not got[1].any() and not got[2].any()
+    assert_device_healthy()
+
+
+def test_copies_and_pickles_leave_the_plans_behind():
+    layer = make(96, 64)
+    x = randn((70, 96), 1).cuda()
+    layer(x.requires_grad_()).sum().backward()
+    want = layer(x)
+    buffer = io.BytesIO()
+    torch.save(layer, buffer)
+    buffer.seek(0)
+    for other in (copy.deepcopy(layer), torch.load(buffer, weights_only=False)):
+        assert torch.equal(other(x), want)
+
+
+def test_the_sparsity_optimizer_moves_blocks_of_the_layer():
+    layer = make(128, 256, density=0.25)
+    x, dh = randn((100, 128), 1).cuda(), randn((100, 256), 2).cuda()
+    sparse = SparseOptimizer(SparseOptimizer.sparse_objects(layer), lr=0.25, new_coefficients_scale=1.0, seed=1)
+    adam = torch.optim.Adam(layer.parameters(), lr=1e-3)
+    sparse.attach_optimizer(adam)
+    layer(x).backward(dh)  # plans exist before the pattern changes
+    before = layer.weight.to_dense().detach().clone()
+    adam.step()
+    sparse.step()
+    assert not torch.equal(before != 0, layer.weight.to_dense().detach() != 0)
+    xs = x.clone().requires_grad_()
+    h = layer(xs)
+    dx, dw = torch.autograd.grad(h, [xs, layer.weight.data], dh)
+    want = reference(layer, x, dh)
+    assert rel(h, want[0]) <= 1e-5 and rel(dx, want[1]) <= 1e-5 and rel(dw, in_data_layout(layer, want[2])) <= 1e-5
+
+
 def test_from_linears_and_state_dict():
     torch.manual_seed(0)
     gate, up = torch.nn.Linear(96, 64), torch.nn.Linear(96, 64)
@@ -492,14 +535,16 @@ def test_a_feed_forward_block_trains_and_serves():
         down.bias.normal_(0, 0.1)
     x, dy = randn((2, 35, 128), 1), randn((2, 35, 128), 2)
     xg = x.cuda().requires_grad_()
-    seed = down.dropout_rng.tolist()[0]
+    torch.manual_seed(4)
+    seed, counter = torch.randint(1 << 62, (2,), device="cuda").tolist()
+    torch.manual_seed(4)
     out = down(up(xg), residual=xg)
     leaves = [xg, up.weight.data, up.bias, down.weight.data, down.bias]
     got = torch.autograd.grad(out, leaves, dy.cuda())
     # 64 bits, by autograd on the host
     from .test_dropout_gpu import philox_halves
 
-    keep = torch.from_numpy(philox_halves(out.numel(), seed, 0) >= round(0.2 * 65536)).view(70, 128)
+    keep = torch.from_numpy(philox_halves(out.numel(), seed, counter) >= round(0.2 * 65536)).view(70, 128)
     host = [x.double().reshape(-1, 128), up.weight.to_dense().detach().cpu().double(), up.bias.detach().cpu().double(),
             down.weight.to_dense().detach().cpu().double(), down.bias.detach().cpu().double()]
     host = [t.requires_grad_() for t in host]
