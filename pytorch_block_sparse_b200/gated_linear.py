@@ -57,20 +57,28 @@ class BlockSparseGatedFunction(torch.autograd.Function):
         return h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        input, pre, data = ctx.saved_tensors
-        weight, (want_x, want_w, _, want_bias, _, _) = ctx.weight, ctx.needs_input_grad
-        grad = grad.contiguous()
-        if grad.dtype is torch.bfloat16 and (grad.shape[0] < 32 or data.shape[0] == 0):
-            # the products of bf16 tensors start at 32 tokens: fewer go through the fp32 ones
-            grad, pre = grad.float(), pre.float()
-        x = input if input.dtype is grad.dtype else input.to(grad.dtype)
-        dx, dw, dbias, sumsq = _gated_pass(weight).backward(
-            x, pre, grad, data, ctx.packed, ctx.activation, ctx.precision, want_x, want_w, want_bias)
-        if want_w:
-            weight.last_grad_block_sumsq = sumsq
-        return dx if dx is None or dx.dtype is input.dtype else dx.to(input.dtype), dw, None, dbias, None, None
+        if torch.is_grad_enabled():  # create_graph: the gradients are handed out, a second differentiation raises
+            return _gradients_once(ctx, grad)
+        return _gradients(ctx, grad)
+
+
+def _gradients(ctx, grad):
+    input, pre, data = ctx.saved_tensors
+    weight, (want_x, want_w, _, want_bias, _, _) = ctx.weight, ctx.needs_input_grad
+    grad = grad.contiguous()
+    if grad.dtype is torch.bfloat16 and (grad.shape[0] < 32 or data.shape[0] == 0):
+        # the products of bf16 tensors start at 32 tokens: fewer go through the fp32 ones
+        grad, pre = grad.float(), pre.float()
+    x = input if input.dtype is grad.dtype else input.to(grad.dtype)
+    dx, dw, dbias, sumsq = _gated_pass(weight).backward(
+        x, pre, grad, data, ctx.packed, ctx.activation, ctx.precision, want_x, want_w, want_bias)
+    if want_w:
+        weight.last_grad_block_sumsq = sumsq
+    return dx if dx is None or dx.dtype is input.dtype else dx.to(input.dtype), dw, None, dbias, None, None
+
+
+_gradients_once = once_differentiable(_gradients)
 
 
 def _out_dtype(x, prec):

@@ -469,6 +469,16 @@ def test_no_tokens_with_gradients(precision):
     assert_device_healthy()
 
 
+def test_a_second_differentiation_raises():
+    layer = make(64, 96)
+    x = randn((40, 64), 1).cuda().requires_grad_()
+    want = torch.autograd.grad(layer(x).square().sum(), [x, layer.weight.data])
+    got = torch.autograd.grad(layer(x).square().sum(), [x, layer.weight.data], create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        got[0].sum().backward()
+
+
 def test_copies_and_pickles_leave_the_plans_behind():
     layer = make(96, 64)
     x = randn((70, 96), 1).cuda()
