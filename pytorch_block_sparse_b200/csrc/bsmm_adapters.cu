@@ -126,18 +126,26 @@ __device__ __forceinline__ void multiply(float (*c)[4], const SplitFragment<__nv
         for (int n = 0; n < kN; ++n) mma16816(c[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b[n].hi[s], b[n].hi[s + 1]);
     }
 }
+// fp32: the tensor core truncates its running sums (about 2e-8 per addition), so they only run over this call's inputs.
 template <int kLen, int kN>
 __device__ __forceinline__ void multiply(float (*c)[4], const Fragment<float, kLen>& a0, const Fragment<float, kLen>& a1,
                                          const Fragment<float, kLen> (&b)[kN]) {
+    float sum[kN][4];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
 #pragma unroll
     for (int s = 0; s < kLen; s += 2) {
 #pragma unroll
-        for (int n = 0; n < kN; ++n) mma1688(c[n], a0.lo[s], a1.lo[s], a0.lo[s + 1], a1.lo[s + 1], b[n].hi[s], b[n].hi[s + 1]);
+        for (int n = 0; n < kN; ++n) mma1688(sum[n], a0.lo[s], a1.lo[s], a0.lo[s + 1], a1.lo[s + 1], b[n].hi[s], b[n].hi[s + 1]);
 #pragma unroll
-        for (int n = 0; n < kN; ++n) mma1688(c[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b[n].lo[s], b[n].lo[s + 1]);
+        for (int n = 0; n < kN; ++n) mma1688(sum[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b[n].lo[s], b[n].lo[s + 1]);
 #pragma unroll
-        for (int n = 0; n < kN; ++n) mma1688(c[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b[n].hi[s], b[n].hi[s + 1]);
+        for (int n = 0; n < kN; ++n) mma1688(sum[n], a0.hi[s], a1.hi[s], a0.hi[s + 1], a1.hi[s + 1], b[n].hi[s], b[n].hi[s + 1]);
     }
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[n][e] += sum[n][e];
 }
 template <typename T>
 constexpr int kGroup = sizeof(T) == 2 ? 4 : 2;  // fragments of the right operand held at a time
