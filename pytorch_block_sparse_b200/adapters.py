@@ -124,10 +124,11 @@ class LowRankAdapters(nn.Module):
             if base is None or not base.is_contiguous() or base.data_ptr() % 16 != 0:
                 raise ValueError("inplace wants a contiguous, 16-byte aligned base")
             out = base
+        elif base is not None:
+            base = native._aligned(base.contiguous())
+            out = torch.empty_like(base)
         else:
-            out = torch.empty(lead + (self.out_features,), dtype=kind, device=device)
-            if base is not None:
-                base = native._aligned(base.contiguous())
+            out = x.new_empty(lead + (self.out_features,), dtype=kind)
         if x.dim() != 2:
             x = x.reshape(-1, self.in_features)
         native.adapters(x.contiguous(), requests.offsets, requests.adapters, native._aligned(down), native._aligned(up), scaling,

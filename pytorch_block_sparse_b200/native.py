@@ -702,8 +702,8 @@ class GatedPass:
         flags = precision | (_gated_flags(activation) | (GATED_IO_BF16 if out_dtype is torch.bfloat16 else 0)) << 16
         ws_bytes = lib.bsmm_gated_forward_workspace_bytes(m, k, hidden, csr.nnz, flags) if self.f32 is not None else 0
         whole = ws_bytes > 0  # one kernel for projections, activation and product
-        h = torch.empty((m, hidden), dtype=out_dtype, device=device)
-        pre = torch.empty((m, 2 * hidden), dtype=torch.float32, device=device) if keep or not whole else None
+        h = x.new_empty((m, hidden), dtype=out_dtype)
+        pre = x.new_empty((m, 2 * hidden)) if keep or not whole else None
         plan = packed = ws = None
         if whole:
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
@@ -729,11 +729,11 @@ class GatedPass:
         m, hidden = dh.shape
         k = csc.n_out_blocks * 32
         planes = self.f32 is not None and precision in (PREC_TF32X3, PREC_BF16X3) and m > 0 and csc.nnz > 0
-        dpre = None if planes else torch.empty((m, 2 * hidden), dtype=dh.dtype, device=device)
-        dx = torch.empty((m, k), dtype=dh.dtype, device=device) if want_x else None
+        dpre = None if planes else dh.new_empty((m, 2 * hidden))
+        dx = dh.new_empty((m, k)) if want_x else None
         dw = torch.empty_like(data) if want_w else None
-        sumsq = torch.empty(csc.nnz, dtype=torch.float32, device=device) if want_w else None
-        dbias = torch.empty(2 * hidden, dtype=torch.float32, device=device) if want_bias else None
+        sumsq = data.new_empty(csc.nnz) if want_w else None
+        dbias = data.new_empty(2 * hidden) if want_bias else None
         types = (GATED_IO_BF16 if dh.dtype is torch.bfloat16 else 0) | (GATED_PRE_BF16 if pre.dtype is torch.bfloat16 else 0)
         flags = precision | (_gated_flags(activation) | types) << 16
         ws = torch.empty(max(16, lib.bsmm_gated_backward_workspace_bytes(m, k, hidden, csc.nnz, flags)), dtype=torch.uint8, device=device)
@@ -760,7 +760,7 @@ def gated_small(x, ptr, idx, data, hidden, bias, activation, out_dtype):
     buffers and blocks of the ``2 * hidden``-row matrix."""
     _need_cuda(x, "x")
     m, k = x.shape
-    out = torch.empty((m, hidden), dtype=out_dtype, device=x.device)
+    out = x.new_empty((m, hidden), dtype=out_dtype)
     flags = _gated_flags(activation)
     if x.dtype == torch.bfloat16:
         flags |= GATED_IO_BF16 if out_dtype == torch.bfloat16 else GATED_X_BF16
@@ -824,8 +824,8 @@ def gated_forward(x, plan, data, bias, activation, keep_pre):
     lib = load()
     m = x.shape[0]
     x, data, bias = _aligned(x), _aligned(data), _aligned(bias)
-    h = torch.empty((m, plan.hidden), dtype=torch.bfloat16, device=x.device)
-    pre = torch.empty((m, 2 * plan.hidden), dtype=torch.bfloat16, device=x.device) if keep_pre else None
+    h = x.new_empty((m, plan.hidden))
+    pre = x.new_empty((m, 2 * plan.hidden)) if keep_pre else None
     images = torch.empty(max(16, lib.bsmm_gated_images_bytes(plan.nnz)), dtype=torch.uint8, device=x.device)
     flags = _gated_flags(activation) | GATED_IO_BF16 | GATED_PRE_BF16
     with _on(x.device):
