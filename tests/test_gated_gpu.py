@@ -469,6 +469,29 @@ def test_no_tokens_with_gradients(precision):
     assert_device_healthy()
 
 
+@pytest.mark.parametrize("precision,dtype", [("tf32x3", torch.float32), ("bf16", torch.bfloat16), ("fp32", torch.float32)])
+@pytest.mark.parametrize("tokens", [3, 20, 300])
+def test_non_finite_tokens_stay_alone(precision, dtype, tokens):
+    """A token with a NaN or an infinity loses its own h and dx, every other token's stay bit for bit."""
+    layer = make(160, 96, density=0.6, precision=precision)
+    x, dh = randn((tokens, 160), 1).cuda().to(dtype), randn((tokens, 96), 2).cuda().to(dtype)
+    broken = x.clone()
+    broken[1, ::7] = float("nan")
+    broken[tokens - 1, 3] = float("inf")
+    rest = [t for t in range(tokens) if t not in (1, tokens - 1)]
+    with torch.no_grad():
+        assert torch.equal(layer(broken)[rest], layer(x)[rest])
+        assert torch.isnan(layer(broken)[1]).any()
+    got = []
+    for v in (x, broken):
+        v = v.clone().requires_grad_()
+        h = layer(v)
+        got.append((h.detach(), torch.autograd.grad(h, v, dh)[0]))
+    for a, b in zip(*got):
+        assert torch.equal(a[rest], b[rest])
+    assert_device_healthy()
+
+
 def test_a_second_differentiation_raises():
     layer = make(64, 96)
     x = randn((40, 64), 1).cuda().requires_grad_()
