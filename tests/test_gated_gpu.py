@@ -492,6 +492,56 @@ def test_non_finite_tokens_stay_alone(precision, dtype, tokens):
     assert_device_healthy()
 
 
+@pytest.mark.parametrize("precision,dtype", [("tf32x3", torch.float32), ("bf16", torch.bfloat16)])
+def test_offsets_past_32_bits(precision, dtype):
+    """g and u of more than 2^31 values: the first and last tokens' h and dx, and the weight gradient of a gradient that only they
+    have, against a call on those tokens alone."""
+    tokens, inner, hidden = 270001, 64, 4096
+    layer = make(inner, hidden, density=0.5, precision=precision)
+    x = torch.randn((tokens, inner), device="cuda").to(dtype).requires_grad_()
+    ends = torch.cat([torch.arange(200), torch.arange(tokens - 200, tokens)]).cuda()
+    h = layer(x)
+    dh = torch.zeros_like(h)
+    dh[ends] = torch.randn((400, hidden), device="cuda").to(dtype)
+    dx, dw, db = torch.autograd.grad(h, [x, layer.weight.data, layer.bias], dh)
+    xs = x.detach()[ends].requires_grad_()
+    hs = layer(xs)
+    want = torch.autograd.grad(hs, [xs, layer.weight.data, layer.bias], dh[ends])
+    assert torch.equal(h.detach()[ends], hs.detach()) and torch.equal(dx[ends], want[0])
+    assert not dx[1000:-1000].any()
+    tolerance = 4e-6 if precision == "tf32x3" else 2e-2  # sums in another order (bf16: of rounded terms)
+    assert rel(dw, want[1].cpu().double()) <= tolerance and rel(db, want[2].cpu().double()) <= tolerance
+    assert_device_healthy()
+    del h, dh, x, dx
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("precision,dtype", [("tf32x3", torch.float32), ("bf16", torch.bfloat16)])
+def test_steps_on_two_streams_at_once(precision, dtype):
+    """The first steps of a layer, whose plans the first call builds, on two streams that do not wait for one another."""
+    xs = [randn((700, 1024), i).cuda().to(dtype) for i in range(2)]
+    dh = randn((700, 512), 5).cuda().to(dtype)
+
+    def step(layer, x):
+        x = x.clone().requires_grad_()
+        h = layer(x)
+        return (h.detach(), *torch.autograd.grad(h, [x, layer.weight.data, layer.bias], dh))
+
+    want = [step(make(1024, 512, precision=precision), x) for x in xs]
+    layer = make(1024, 512, precision=precision)
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = []
+    for stream, x in zip(streams, xs):
+        with torch.cuda.stream(stream):
+            got.append([step(layer, x) for _ in range(4)])
+    torch.cuda.synchronize()
+    for rounds, expected in zip(got, want):
+        for values in rounds:
+            assert all(torch.equal(a, b) for a, b in zip(values, expected))
+    assert_device_healthy()
+
+
 def test_a_second_differentiation_raises():
     layer = make(64, 96)
     x = randn((40, 64), 1).cuda().requires_grad_()
